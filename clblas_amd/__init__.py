@@ -43,9 +43,24 @@ class Side(enum.IntEnum):
     Right = 1
 
 
+class Type(enum.IntEnum):
+    """Element types of the feed-forward products (clblasAmdType)."""
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+
+
+class Gate(enum.IntEnum):
+    """Activations of the gated product (clblasAmdGate)."""
+    Silu = 0
+    Gelu = 1
+    GeluTanh = 2
+
+
 class Status(enum.IntEnum):
     Success = 0
     InvalidValue = -30
+    InvalidOperation = -59
     InvalidDevice = -33
     OutOfResources = -5
     OutOfHostMemory = -6
@@ -54,6 +69,8 @@ class Status(enum.IntEnum):
     InvalidMatA = -1022
     InvalidMatB = -1021
     InvalidMatC = -1020
+    InvalidVecX = -1019
+    InvalidVecY = -1018
     InvalidDim = -1017
     InvalidLeadDimA = -1016
     InvalidLeadDimB = -1015
@@ -79,7 +96,8 @@ EXPORTED_SYMBOLS = (
 ) + tuple("clblas%s%s" % (t, f) for f in ("syrk", "trmm", "symm", "syr2k") for t in "SDCZ") + tuple(
     "clblas%s%s" % (t, f) for f in ("herk", "her2k", "hemm") for t in "CZ") + (
     "clblasAmdReleaseStream", "clblasAmdReserveWorkspace", "clblasAmdWorkspaceStats", "clblasAmdLastDispatch",
-    "clblasAmdReloadDebugEnv", "clblasAmdTrsmPollTimeouts", "clblasAmdTileModelQuery", "clblasAmdTileModelParam")
+    "clblasAmdReloadDebugEnv", "clblasAmdTrsmPollTimeouts", "clblasAmdTileModelQuery", "clblasAmdTileModelParam",
+    "clblasAmdQuantizeRows", "clblasAmdI8gemm", "clblasAmdGated", "clblasAmdGatedI8", "clblasAmdGatedGrad")
 
 _lib = None
 
@@ -159,6 +177,15 @@ def _declare(lib):
                                             ctypes.POINTER(ctypes.c_int), ctypes.c_int]
     lib.clblasAmdTileModelParam.restype = ctypes.c_int
     lib.clblasAmdTileModelParam.argtypes = [ctypes.c_char, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_double), ctypes.c_int]
+    m, v = [vp, sz, sz], [vp]  # a matrix (address, offset, leading dimension); a vector
+    for name, types in (("clblasAmdQuantizeRows", [i, sz, sz] + m + m + v),
+                        ("clblasAmdI8gemm", [i, sz, sz, sz] + m + v + m + v + m),
+                        ("clblasAmdGated", [i, i, sz, sz, sz] + 6 * m),
+                        ("clblasAmdGatedI8", [i, i, sz, sz, sz] + 3 * (m + v) + m),
+                        ("clblasAmdGatedGrad", [i, i, sz, sz, sz] + 9 * m)):
+        fn = getattr(lib, name)
+        fn.restype = i
+        fn.argtypes = types + [vp]
     lib.clblasAmdTrsmPollTimeouts.restype = ctypes.c_int
     lib.clblasAmdTrsmPollTimeouts.argtypes = [ctypes.POINTER(ctypes.c_uint), ctypes.c_int]
 
@@ -414,3 +441,42 @@ def hemm(prefix, order, side, uplo, M, N, alpha, A, offA, lda, B, offB, ldb, bet
     fn = getattr(load_library(), "clblas%shemm" % prefix)
     return fn(int(order), int(side), int(uplo), M, N, _scalar(prefix, alpha), _ptr(A), offA, lda, _ptr(B), offB, ldb,
               _scalar(prefix, beta), _ptr(C), offC, ldc, _stream(stream))
+
+
+# ---- the products of a gated feed-forward layer (row-major; include/clblas_amd.h) ----
+
+def quantize_rows(type_, M, K, X, offX, ldx, Q, offQ, ldq, scale, stream=None):
+    """clblasAmdQuantizeRows: rows of X (Type) to 8-bit integers Q with one scale each."""
+    return load_library().clblasAmdQuantizeRows(int(type_), M, K, _ptr(X), offX, ldx, _ptr(Q), offQ, ldq, _ptr(scale),
+                                                _stream(stream))
+
+
+def i8gemm(typeC, M, N, K, A, offA, lda, scaleA, B, offB, ldb, scaleB, C, offC, ldc, stream=None):
+    """clblasAmdI8gemm: C = diag(scaleA) A B^T diag(scaleB), A and B 8-bit, C of typeC (Type)."""
+    return load_library().clblasAmdI8gemm(int(typeC), M, N, K, _ptr(A), offA, lda, _ptr(scaleA), _ptr(B), offB, ldb,
+                                          _ptr(scaleB), _ptr(C), offC, ldc, _stream(stream))
+
+
+def gated(type_, gate, M, N, K, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, H, offH, ldh, G=None, offG=0, ldg=0,
+          U=None, offU=0, ldu=0, stream=None):
+    """clblasAmdGated: H = act(X Wg^T) o (X Wu^T); G and U (both or neither) receive the two products."""
+    return load_library().clblasAmdGated(int(type_), int(gate), M, N, K, _ptr(X), offX, ldx, _ptr(Wg), offWg, ldwg,
+                                         _ptr(Wu), offWu, ldwu, _ptr(H), offH, ldh, _ptr(G), offG, ldg, _ptr(U), offU,
+                                         ldu, _stream(stream))
+
+
+def gated_i8(typeH, gate, M, N, K, X, offX, ldx, scaleX, Wg, offWg, ldwg, scaleWg, Wu, offWu, ldwu, scaleWu, H, offH,
+             ldh, stream=None):
+    """clblasAmdGatedI8: the gated product on 8-bit operands with scales, H of typeH (Type)."""
+    return load_library().clblasAmdGatedI8(int(typeH), int(gate), M, N, K, _ptr(X), offX, ldx, _ptr(scaleX), _ptr(Wg),
+                                           offWg, ldwg, _ptr(scaleWg), _ptr(Wu), offWu, ldwu, _ptr(scaleWu), _ptr(H),
+                                           offH, ldh, _stream(stream))
+
+
+def gated_grad(type_, gate, M, N, K, dH, offdH, lddh, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, G, offG, ldg, U,
+               offU, ldu, dX, offdX, lddx, dWg, offdWg, lddwg, dWu, offdWu, lddwu, stream=None):
+    """clblasAmdGatedGrad: dX (or None), dWg and dWu (or both None) from dH, the operands and the stored G and U."""
+    return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, _ptr(dH), offdH, lddh, _ptr(X), offX, ldx,
+                                             _ptr(Wg), offWg, ldwg, _ptr(Wu), offWu, ldwu, _ptr(G), offG, ldg, _ptr(U),
+                                             offU, ldu, _ptr(dX), offdX, lddx, _ptr(dWg), offdWg, lddwg, _ptr(dWu),
+                                             offdWu, lddwu, _stream(stream))

@@ -331,6 +331,75 @@ clblasStatus clblasZhemm(clblasOrder order, clblasSide side, clblasUplo uplo, si
                          const DoubleComplex *B, size_t offB, size_t ldb, DoubleComplex beta,
                          DoubleComplex *C, size_t offC, size_t ldc, hipStream_t stream); /* src/clBLAS.h:9305-9326 */
 
+/* ---- The products of a gated feed-forward layer.  No counterpart in the reference, which has no type below 32 bits.
+ * All matrices are row-major: a row of X, H, dH, dX is one token, a row of a weight one channel (the layout in which
+ * a linear layer keeps them), `ld` counts the elements from one row to the next, and element offsets are added to the
+ * pointers as everywhere in this library.  (Column-major callers of the 8-bit product exchange A with B and M with N: the
+ * row-major result of that call is theirs.)  Elements need only the alignment of their type; rows whose addresses
+ * and lengths are multiples of 16 bytes spare a copy of that operand into the stream's trmm buffer.  Sums are held
+ * in 32 bits - float, or int32 for 8-bit operands - and every result is rounded once, to nearest.  Results must not
+ * overlap operands or each other.
+ * Checks, in this order: null matrices (X, A: clblasInvalidMatA, weights and other operands: ...MatB, results: ...MatC),
+ * null scales (clblasInvalidVecX for tokens, ...VecY for channels), types and gates that do not exist or that the call
+ * does not take (clblasInvalidValue), zero dimensions (clblasInvalidDim), then leading dimensions, in the order of the
+ * arguments (clblasInvalidLeadDim{A,B,C}). ---- */
+
+typedef enum clblasAmdType_ CLBLAS_AMD_ENUM_BASE {
+    clblasAmdF32 = 0,
+    clblasAmdF16 = 1,
+    clblasAmdBf16 = 2
+} clblasAmdType;
+
+/* act(g): g / (1 + exp(-g));  g Phi(g), Phi the normal distribution;  its tanh form
+ * g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+typedef enum clblasAmdGate_ CLBLAS_AMD_ENUM_BASE {
+    clblasAmdSilu = 0,
+    clblasAmdGelu = 1,
+    clblasAmdGeluTanh = 2
+} clblasAmdGate;
+
+/* Rows to 8-bit integers with one scale each:
+ *   a_i = max_k |X(i,k)|,  scale(i) = a_i / 127,  Q(i,k) = round(127 X(i,k) / a_i), ties to even, exactly.
+ * X and Q are M x K; `type` is X's.  A row of zeros gives zeros and scale 0; a row that holds NaN or an infinity gives
+ * zeros and that as its scale, so that products with it come out as NaN.  Elements of Q's rows beyond K keep their values. */
+clblasStatus clblasAmdQuantizeRows(clblasAmdType type, size_t M, size_t K, const void *X, size_t offX, size_t ldx,
+                                   signed char *Q, size_t offQ, size_t ldq, float *scale, hipStream_t stream);
+
+/* 8-bit product with a scale for each token and each channel:
+ *   C(m,n) = scaleA(m) scaleB(n) sum_k A(m,k) B(n,k)
+ * A is M x K, B is N x K (both 8-bit), C is M x N of `typeC`.  The integer sum is exact; K beyond 131071, where it could
+ * pass 31 bits, is refused with clblasNotImplemented. */
+clblasStatus clblasAmdI8gemm(clblasAmdType typeC, size_t M, size_t N, size_t K,
+                             const signed char *A, size_t offA, size_t lda, const float *scaleA,
+                             const signed char *B, size_t offB, size_t ldb, const float *scaleB,
+                             void *C, size_t offC, size_t ldc, hipStream_t stream);
+
+/* Gated product:  G = X Wg^T,  U = X Wu^T,  H = act(G) o U  (o: element by element, on the unrounded sums)
+ * X is M x K, Wg and Wu are N x K, H, G and U are M x N, all of `type` (F16 or Bf16).  G and U, which the gradients need,
+ * are stored if their pointers are given: both or neither (one alone: clblasInvalidMatC). */
+clblasStatus clblasAmdGated(clblasAmdType type, clblasAmdGate gate, size_t M, size_t N, size_t K,
+                            const void *X, size_t offX, size_t ldx, const void *Wg, size_t offWg, size_t ldwg,
+                            const void *Wu, size_t offWu, size_t ldwu, void *H, size_t offH, size_t ldh,
+                            void *G, size_t offG, size_t ldg, void *U, size_t offU, size_t ldu, hipStream_t stream);
+
+/* The gated product on 8-bit operands (as clblasAmdI8gemm's), H of `typeH`. */
+clblasStatus clblasAmdGatedI8(clblasAmdType typeH, clblasAmdGate gate, size_t M, size_t N, size_t K,
+                              const signed char *X, size_t offX, size_t ldx, const float *scaleX,
+                              const signed char *Wg, size_t offWg, size_t ldwg, const float *scaleWg,
+                              const signed char *Wu, size_t offWu, size_t ldwu, const float *scaleWu,
+                              void *H, size_t offH, size_t ldh, hipStream_t stream);
+
+/* Gradients of the gated product from dH, its operands and the G and U it stored:
+ *   dU = dH o act(G),  dG = dH o U o act'(G);   dX = dG Wg + dU Wu,   dWg = dG^T X,   dWu = dU^T X
+ * all of `type` (F16 or Bf16).  dG and dU pass through the stream's trmm buffer, rounded to `type` once.  dX may be null (it
+ * is not computed), and so may dWg and dWu together; all three null, or one of dWg and dWu alone, is clblasInvalidMatC. */
+clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M, size_t N, size_t K,
+                                const void *dH, size_t offdH, size_t lddh, const void *X, size_t offX, size_t ldx,
+                                const void *Wg, size_t offWg, size_t ldwg, const void *Wu, size_t offWu, size_t ldwu,
+                                const void *G, size_t offG, size_t ldg, const void *U, size_t offU, size_t ldu,
+                                void *dX, size_t offdX, size_t lddx, void *dWg, size_t offdWg, size_t lddwg,
+                                void *dWu, size_t offdWu, size_t lddwu, hipStream_t stream);
+
 /* ---- Workspace and diagnostics.  These four have no counterpart in the reference: clBLAS allocates
  * and frees its temporaries inside every call (src/library/blas/xtrsm.cc:1186-1207, 1499-1500) and
  * logs nothing; this library keeps scratch buffers per (device, stream) and lets the caller
