@@ -50,6 +50,8 @@ void read_knobs() {
     k.stagger = env_int("CLBLAS_AMD_GEMM_STAGGER", 1);
     k.deep_panels = env_int("CLBLAS_AMD_GEMM_DEEP", 1);
     k.wide_ld = env_int("CLBLAS_AMD_GEMM_WIDE_LD", 0);
+    k.ffn_form = env_int("CLBLAS_AMD_FFN_FORM", -1);
+    k.ffn_splits = env_int("CLBLAS_AMD_FFN_SPLITS", 0);
     k.log = env_int("CLBLAS_AMD_LOG", 0);
     k.check_mem = env_int("CLBLAS_AMD_CHECK_MEM", 0);
     k.trsm_leaf = env_int("CLBLAS_AMD_TRSM_LEAF", 0);

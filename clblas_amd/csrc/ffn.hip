@@ -121,56 +121,47 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const char *from, int64_
     }
 }
 
-// 16-bit matrix, rows x cols -> its transpose: cols rows of ld_to elements, zeros behind the first `rows` of them.
-__global__ __launch_bounds__(256) void transpose_kernel(const uint16_t *from, int64_t ld, int rows, int cols, uint16_t *to, int64_t ld_to) {
-    __shared__ uint16_t tile[64][65];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4) tile[i][x] = (r0 + i < rows && c0 + x < cols) ? from[(int64_t)(r0 + i) * ld + c0 + x] : (uint16_t)0;
-    __syncthreads();
-    for (int i = y; i < 64; i += 4)
-        if (c0 + i < cols && r0 + x < ld_to) to[(int64_t)(c0 + i) * ld_to + r0 + x] = tile[x][i];
-}
-
 // ---- gradients of the gate ----
 //
 // dG = dH o U o act'(G), dU = dH o act(G), rounded to the operands' 16 bits as the two products that follow take
 // them (each result below sums many of them: the roundings, independent and unbiased, add up to about one more
-// rounding of the result).  Written twice: rows of tokens [dG | dU], zeros from N to ld_half, for dX, and rows of channels
-// (transposed, zeros behind M) for dWg and dWu.
+// rounding of the result).  A row per token, [dG | dU], either half padded with zeros to a multiple of 64.
 template <int OT> __global__ __launch_bounds__(256) void gate_grad_kernel(const void *dH_, int64_t lddh, const void *G_, int64_t ldg, const void *U_,
-                                                                          int64_t ldu, int M, int N, int gate, void *out_, int64_t ld_half,
-                                                                          void *outT_, int64_t ldT) {
+                                                                          int64_t ldu, int M, int N, int gate, void *out_, int64_t half) {
     typedef typename Store<OT>::type T;
+    struct Vec8 { T v[8]; };
     const T *dH = static_cast<const T *>(dH_), *G = static_cast<const T *>(G_), *U = static_cast<const T *>(U_);
-    T *out = static_cast<T *>(out_), *outT = static_cast<T *>(outT_);
-    __shared__ T tile[2][64][66];
-    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4) {
-        const int m = m0 + i, n = n0 + x;
-        float dg = 0.f, du = 0.f;
-        if (m < M && n < N) {
+    T *out = static_cast<T *>(out_);
+    const int64_t per_row = half >> 3, total = per_row * M;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+        const int64_t m = t / per_row;
+        const int n = (int)(t - m * per_row) * 8;
+        const T *h = dH + m * lddh + n, *g = G + m * ldg + n, *u = U + m * ldu + n;
+        Vec8 vh = {}, vg = {}, vu = {}, dg, du;
+        if (n + 8 <= N) {
+            __builtin_memcpy(&vh, h, 16);
+            __builtin_memcpy(&vg, g, 16);
+            __builtin_memcpy(&vu, u, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < N) {
+                    vh.v[e] = h[e];
+                    vg.v[e] = g[e];
+                    vu.v[e] = u[e];
+                }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
             float act, slope;
-            gate_value_and_slope(gate, (float)G[(int64_t)m * ldg + n], act, slope);
-            const float dh = (float)dH[(int64_t)m * lddh + n];
-            du = dh * act;
-            dg = dh * (float)U[(int64_t)m * ldu + n] * slope;
+            gate_value_and_slope(gate, (float)vg.v[e], act, slope);
+            const float dh = (float)vh.v[e];
+            dg.v[e] = Store<OT>::of(dh * (float)vu.v[e] * slope);
+            du.v[e] = Store<OT>::of(dh * act);
         }
-        const T tg = Store<OT>::of(dg), tu = Store<OT>::of(du);
-        if (m < M && n < ld_half && out) {
-            out[(int64_t)m * 2 * ld_half + n] = tg;
-            out[(int64_t)m * 2 * ld_half + ld_half + n] = tu;
-        }
-        tile[0][i][x] = tg;
-        tile[1][i][x] = tu;
-    }
-    __syncthreads();
-    if (!outT) return;
-    for (int i = y; i < 64; i += 4) {
-        const int n = n0 + i, m = m0 + x;
-        if (n < N && m < ldT) {
-            outT[(int64_t)n * ldT + m] = tile[0][x][i];
-            outT[((int64_t)N + n) * ldT + m] = tile[1][x][i];
-        }
+        T *to = out + m * 2 * half + n;
+        __builtin_memcpy(__builtin_assume_aligned(to, 16), &dg, 16);
+        __builtin_memcpy(__builtin_assume_aligned(to + half, 16), &du, 16);
     }
 }
 
@@ -205,18 +196,37 @@ hipError_t launched(const char *kernel, char type, int bm, int bn, int threads, 
 char type_letter(int et) { return et == ET_I8 ? 'i' : et == ET_F16 ? 'h' : 'b'; }
 
 template <typename Cfg> hipError_t launch_tiles(const Product &p, int K, hipStream_t stream) {
-    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
-    if (grid * Cfg::THREADS > 0xffffffffLL) return hipErrorNotSupported;
-    if (Cfg::LDS > 65536) {
-        hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<Cfg>, Cfg::LDS);
-        if (e != hipSuccess) return e;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
+    if (tiles > 0x7fffffff - 65536) return hipErrorNotSupported;
+    // as many workgroups as the card holds at once
+    const int per_cu = 160 * 1024 / Cfg::LDS < 8 / Cfg::WAVES ? 160 * 1024 / Cfg::LDS : 8 / Cfg::WAVES;
+    const unsigned grid = (unsigned)(tiles < 256 * per_cu ? tiles : 256 * per_cu);
+    hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<Cfg>, Cfg::LDS);
+    if (e != hipSuccess) return e;
+    e = launch_kernel(tile_kernel<Cfg>, dim3(grid), dim3(Cfg::THREADS), Cfg::LDS, stream, p);
+    return launched("ffn_tile_kernel", type_letter(Cfg::ET), Cfg::BM, Cfg::CHANNELS, Cfg::THREADS, p.M, p.N, K, grid, 1, p.splits, e);
+}
+
+// The tiled forms: edges, and the index by which a form is known (the forms that run from registers come first).
+enum { ROWS_FORMS = 6 };
+struct TileShape { int bm, bn; };
+const TileShape kTiles[] = {{256, 256}, {256, 256}, {128, 128}, {128, 256}, {64, 128}, {128, 64}, {64, 64}, {256, 128}};
+
+template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
+    switch (tile) {
+    case 0: return f(TileCfg<ET, 256, 256, 128, 64, 5, GATED, LA, LB>());
+    case 1: return f(TileCfg<ET, 256, 256, 128, 64, 4, GATED, LA, LB>());
+    case 2: return f(TileCfg<ET, 128, 128, 64, 64, 5, GATED, LA, LB>());
+    case 3: return f(TileCfg<ET, 128, 256, 64, 64, 6, GATED, LA, LB>());
+    case 4: return f(TileCfg<ET, 64, 128, 32, 64, 6, GATED, LA, LB>());
+    case 5: return f(TileCfg<ET, 128, 64, 64, 32, 6, GATED, LA, LB>());
+    case 6: return f(TileCfg<ET, 64, 64, 32, 32, 8, GATED, LA, LB>());
+    default: return f(TileCfg<ET, 256, 128, 64, 64, 6, GATED, LA, LB>());
     }
-    hipError_t e = launch_kernel(tile_kernel<Cfg>, dim3((unsigned)grid), dim3(Cfg::THREADS), Cfg::LDS, stream, p);
-    return launched("ffn_tile_kernel", type_letter(Cfg::ET), Cfg::BM, Cfg::CHANNELS, Cfg::THREADS, p.M, p.N, K, (unsigned)grid, 1, p.splits, e);
 }
 
 struct TileChoice {
-    int big = 0, bm = 0, channels = 0, tiles_m = 0, tiles_n = 0, splits = 1, steps_per_split = 0;
+    int tile = 0, tiles_m = 0, tiles_n = 0, splits = 1, steps_per_split = 0;
     int64_t ws_ld = 0, ws_plane = 0, ws_split = 0;
     size_t ws_bytes = 0;
 };
@@ -226,21 +236,22 @@ struct TileChoice {
 TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
     TileChoice c;
     const int64_t steps = ceil_div(k_bytes, 128);
-    auto tiles = [&](int edge) { return ceil_div(M, edge) * ceil_div(N, gated ? edge / 2 : edge) * batch; };
-    c.big = tiles(256) >= 256;
-    c.bm = c.big ? 256 : 128;
-    c.channels = gated ? c.bm / 2 : c.bm;
-    c.tiles_m = (int)ceil_div(M, c.bm);
-    c.tiles_n = (int)ceil_div(N, c.channels);
+    auto tiles = [&](int bm, int bn) { return ceil_div(M, bm) * ceil_div(N, gated ? bn / 2 : bn) * batch; };
+    c.tile = tiles(256, 256) >= 256 ? 0 : 2;
+    if (knobs().ffn_form >= ROWS_FORMS) c.tile = knobs().ffn_form - ROWS_FORMS;
+    const TileShape t = kTiles[c.tile];
+    c.tiles_m = (int)ceil_div(M, t.bm);
+    c.tiles_n = (int)ceil_div(N, gated ? t.bn / 2 : t.bn);
     int64_t splits = 1;
-    if (!c.big) {
-        splits = 512 / tiles(128);
+    if (t.bm * t.bn < 65536) {
+        splits = 512 / tiles(t.bm, t.bn);
         if (splits > steps / 4) splits = steps / 4;
         if (splits > 64) splits = 64;
-        if (splits < 1) splits = 1;
     }
-    c.steps_per_split = (int)ceil_div(steps, splits);
-    c.splits = (int)ceil_div(steps, c.steps_per_split);
+    if (knobs().ffn_splits) splits = knobs().ffn_splits < steps ? knobs().ffn_splits : steps;
+    if (splits < 1) splits = 1;
+    c.steps_per_split = 2 * (int)ceil_div(steps, splits);
+    c.splits = (int)ceil_div(2 * steps, c.steps_per_split);
     if (c.splits > 1) {
         c.ws_ld = round_up(N, 4);
         c.ws_plane = c.ws_ld * M;
@@ -250,7 +261,7 @@ TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
     return c;
 }
 
-template <int ET, bool GATED> hipError_t run_product(Product p, const TileChoice &c, uint32_t *ws, int K, hipStream_t stream) {
+template <int ET, bool GATED, Lay LA, Lay LB> hipError_t run_product(Product p, const TileChoice &c, uint32_t *ws, int K, hipStream_t stream) {
     p.tiles_m = c.tiles_m;
     p.tiles_n = c.tiles_n;
     p.group_m = 8;
@@ -260,14 +271,36 @@ template <int ET, bool GATED> hipError_t run_product(Product p, const TileChoice
     p.ws_ld = c.ws_ld;
     p.ws_plane = c.ws_plane;
     p.ws_split = c.ws_split;
-    hipError_t e;
-    if (c.big) e = launch_tiles<TileCfg<ET, 16, 256, 256, 128, 64, GATED>>(p, K, stream);
-    else e = launch_tiles<TileCfg<ET, 16, 128, 128, 64, 64, GATED>>(p, K, stream);
+    hipError_t e = with_tile<ET, GATED, LA, LB>(c.tile, [&](auto cfg) { return launch_tiles<decltype(cfg)>(p, K, stream); });
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t work = (c.ws_ld >> 2) * p.M * p.batch;
     const unsigned grid = (unsigned)(ceil_div(work, 256) < 2048 ? ceil_div(work, 256) : 2048);
     e = launch_kernel(join_kernel<ET, GATED>, dim3(grid), dim3(256), 0, stream, p);
     return launched("ffn_join_kernel", type_letter(ET), 1, 4, 256, p.M, p.N, K, grid, 1, p.splits, e);
+}
+
+template <typename Cfg> hipError_t launch_rows(Product p, int K, hipStream_t stream) {
+    p.tiles_m = (int)ceil_div(p.M, 16 * Cfg::TM);
+    p.tiles_n = (int)ceil_div(p.N, 16 * Cfg::TN);
+    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
+    if (grid * Cfg::THREADS > 0xffffffffLL) return hipErrorNotSupported;
+    if (Cfg::LDS > 65536) {
+        hipError_t e = ensure_dynamic_lds((const void *)rows_kernel<Cfg>, Cfg::LDS);
+        if (e != hipSuccess) return e;
+    }
+    hipError_t e = launch_kernel(rows_kernel<Cfg>, dim3((unsigned)grid), dim3(Cfg::THREADS), Cfg::LDS, stream, p);
+    return launched("ffn_rows_kernel", type_letter(Cfg::ET), 16 * Cfg::TM, 16 * Cfg::TN, Cfg::THREADS, p.M, p.N, K, (unsigned)grid, 1, 1, e);
+}
+
+template <int ET, bool GATED> hipError_t run_rows(const Product &p, int form, int K, hipStream_t stream) {
+    switch (form) {
+    case 0: return launch_rows<RowsCfg<ET, 1, 1, 8, 4, GATED>>(p, K, stream);
+    case 1: return launch_rows<RowsCfg<ET, 2, 1, 8, 4, GATED>>(p, K, stream);
+    case 2: return launch_rows<RowsCfg<ET, 2, 2, 8, 2, GATED>>(p, K, stream);
+    case 3: return launch_rows<RowsCfg<ET, 4, 1, 8, 2, GATED>>(p, K, stream);
+    case 4: return launch_rows<RowsCfg<ET, 4, 2, 4, 2, GATED>>(p, K, stream);
+    default: return launch_rows<RowsCfg<ET, 4, GATED ? 2 : 4, 4, 2, GATED>>(p, K, stream);
+    }
 }
 
 // Layout of one call's copies in the stream's buffer.
@@ -280,10 +313,10 @@ struct Copies {
     }
 };
 
-// Whether the tiled product can load an operand from where it is: 16 bytes at a time along k, from dword-aligned
-// addresses, rows near enough for 32-bit offsets across a tile.
-bool fits(const void *ptr, int64_t ld_bytes, int64_t k_bytes) {
-    return (reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && (ld_bytes & 3) == 0 && (k_bytes & 15) == 0 && ld_bytes < ((int64_t)1 << 22);
+// Whether the tiled product can load an operand from where it is: dword-aligned rows, near enough to each other for 32-bit
+// offsets across a tile.
+bool fits(const void *ptr, int64_t ld_bytes) {
+    return (reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && (ld_bytes & 3) == 0 && ld_bytes < ((int64_t)1 << 22);
 }
 
 hipError_t pack_rows(const void *from, int64_t ld, int64_t bytes, char *to, int64_t ld_to, int64_t rows, hipStream_t stream) {
@@ -298,18 +331,32 @@ template <int ET, bool GATED>
 hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Product p, hipStream_t stream) {
     const int64_t kb = (int64_t)K * es, kp = round_up(kb, 16);
     Mat in[3] = {A, B0, B1};
+    const int form = knobs().ffn_form;
+    if (form >= 0 && form < ROWS_FORMS) {
+        p.A[0] = A.ptr;
+        p.lda = A.ld * es;
+        p.B[0] = B0.ptr;
+        p.B[1] = B1.ptr;
+        p.ldb[0] = B0.ld * es;
+        p.ldb[1] = B1.ld * es;
+        p.k_bytes = kb;
+        p.M = M;
+        p.N = N;
+        p.batch = 1;
+        return run_rows<ET, GATED>(p, form, K, stream);
+    }
     const int64_t rows[3] = {M, N, N};
     size_t at[3] = {0, 0, 0};
     bool copy[3] = {false, false, false};
     Copies copies;
     for (int i = 0; i < (GATED ? 3 : 2); ++i) {
-        copy[i] = !fits(in[i].ptr, in[i].ld * es, kb);
+        copy[i] = !fits(in[i].ptr, in[i].ld * es);
         if (copy[i]) at[i] = copies.add((size_t)kp * rows[i]);
     }
     char *buf = nullptr;
     hipError_t e;
     if (copies.used && (e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf)) != hipSuccess) return e;
-    const TileChoice c = choose(GATED, M, N, 1, kp);
+    const TileChoice c = choose(GATED, M, N, 1, kb);
     uint32_t *ws = nullptr;
     if (c.ws_bytes && (e = workspace_get(stream, c.ws_bytes, WS_GEMM, (void **)&ws)) != hipSuccess) return e;
     const void *ptr[3];
@@ -333,30 +380,32 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
         p.ldb[h] = ld[i];
         p.b_bytes[h] = bytes[i];
     }
-    p.k_bytes = kp;
+    p.k_bytes = kb;
     p.M = M;
     p.N = N;
     p.batch = 1;
-    return run_product<ET, GATED>(p, c, ws, K, stream);
-}
-
-hipError_t transpose(const void *from, int64_t ld, int rows, int cols, void *to, int64_t ld_to, int64_t rows_padded, hipStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(rows_padded, 64), (unsigned)ceil_div(cols, 64));
-    hipError_t e = launch_kernel(transpose_kernel, grid, dim3(256), 0, stream, (const uint16_t *)from, ld, rows, cols, (uint16_t *)to, ld_to);
-    return launched("ffn_transpose_kernel", 'p', 64, 64, 256, rows, cols, 0, grid.x, grid.y, 1, e);
+    p.part_steps = 0x7fffffff;
+    return run_product<ET, GATED, ALONG_K, ALONG_K>(p, c, ws, K, stream);
 }
 
 template <int ET, int OT>
 hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu, Mat G, Mat U, OutMat dX, OutMat dWg, OutMat dWu,
                    hipStream_t stream) {
-    const int64_t Np = round_up(N, 64), Mp = round_up(M, 8);
+    const int64_t half = round_up(N, 64), row = 2 * half * 2;  // [dG | dU]: elements to dU, bytes to the next token
     const bool want_x = dX.ptr, want_w = dWg.ptr;
+    // operands that the tiles load as they are, or copies
+    Mat in[3] = {X, Wg, Wu};
+    const int64_t rows[3] = {M, N, N}, ld_copy = round_up((int64_t)K * 2, 16);
+    const bool used[3] = {want_w, want_x, want_x};
     Copies copies;
-    const size_t at_rows = want_x ? copies.add((size_t)M * 2 * Np * 2) : 0;
-    const size_t at_wt = want_x ? copies.add((size_t)K * 2 * Np * 2) : 0;
-    const size_t at_cols = want_w ? copies.add((size_t)2 * N * Mp * 2) : 0;
-    const size_t at_xt = want_w ? copies.add((size_t)K * Mp * 2) : 0;
-    const TileChoice cx = choose(false, M, K, 1, 2 * Np * 2), cw = choose(false, N, K, 2, Mp * 2);
+    const size_t at_grads = copies.add((size_t)M * row);
+    size_t at[3] = {0, 0, 0};
+    bool copy[3];
+    for (int i = 0; i < 3; ++i) {
+        copy[i] = used[i] && !fits(in[i].ptr, in[i].ld * 2);
+        if (copy[i]) at[i] = copies.add((size_t)rows[i] * ld_copy);
+    }
+    const TileChoice cx = choose(false, M, K, 1, row), cw = choose(false, N, K, 2, (int64_t)M * 2);
     size_t sums = want_x ? cx.ws_bytes : 0;
     if (want_w && cw.ws_bytes > sums) sums = cw.ws_bytes;
     char *buf = nullptr;
@@ -364,36 +413,48 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     hipError_t e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf);
     if (e == hipSuccess && sums) e = workspace_get(stream, sums, WS_GEMM, (void **)&ws);
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)ceil_div(M, 64), (unsigned)ceil_div(N, 64));
-    e = launch_kernel(gate_grad_kernel<OT>, grid, dim3(256), 0, stream, dH.ptr, dH.ld, G.ptr, G.ld, U.ptr, U.ld, M, N, gate,
-                      want_x ? buf + at_rows : nullptr, Np, want_w ? buf + at_cols : nullptr, Mp);
-    if ((e = launched("ffn_gate_grad_kernel", type_letter(ET), 64, 64, 256, M, N, K, grid.x, grid.y, 1, e)) != hipSuccess) return e;
+    char *grads = buf + at_grads;
+    const void *ptr[3];
+    int64_t ld[3];
+    for (int i = 0; i < 3; ++i) {
+        ptr[i] = copy[i] ? buf + at[i] : in[i].ptr;
+        ld[i] = copy[i] ? ld_copy : in[i].ld * 2;
+        if (copy[i] && (e = pack_rows(in[i].ptr, in[i].ld * 2, (int64_t)K * 2, buf + at[i], ld_copy, rows[i], stream)) != hipSuccess) return e;
+    }
+    const int64_t work = M * (half / 8);
+    const unsigned grid = (unsigned)(ceil_div(work, 256) < 8192 ? ceil_div(work, 256) : 8192);
+    e = launch_kernel(gate_grad_kernel<OT>, dim3(grid), dim3(256), 0, stream, dH.ptr, dH.ld, G.ptr, G.ld, U.ptr, U.ld, M, N, gate, (void *)grads, half);
+    if ((e = launched("ffn_gate_grad_kernel", type_letter(ET), 1, 8, 256, M, N, K, grid, 1, 1, e)) != hipSuccess) return e;
     Product p = {};
     p.out_type = OT;
-    if (want_x) {
-        uint16_t *wt = (uint16_t *)(buf + at_wt);
-        if ((e = transpose(Wg.ptr, Wg.ld, N, K, wt, 2 * Np, Np, stream)) != hipSuccess) return e;
-        if ((e = transpose(Wu.ptr, Wu.ld, N, K, wt + Np, 2 * Np, Np, stream)) != hipSuccess) return e;
-        p.A[0] = p.A[1] = buf + at_rows;
-        p.B[0] = p.B[1] = wt;
-        p.lda = p.ldb[0] = p.ldb[1] = p.k_bytes = 2 * Np * 2;
-        p.a_bytes = M * p.lda;
-        p.b_bytes[0] = p.b_bytes[1] = K * p.lda;
+    p.lda = row;
+    if (want_x) {  // [dG | dU] (M x 2 half) times [Wg; Wu]: the depth runs through Wg's rows, then through Wu's
+        p.A[0] = p.A[1] = grads;
+        p.a_bytes = M * row;
+        for (int h = 0; h < 2; ++h) {
+            p.B[h] = ptr[1 + h];
+            p.ldb[h] = ld[1 + h];
+            p.b_bytes[h] = (N - 1) * ld[1 + h] + (int64_t)K * 2;
+        }
+        p.k_bytes = row;
+        p.part_steps = (int)(half / 32);
         p.C[0] = p.C[1] = dX.ptr;
         p.ldc[0] = p.ldc[1] = dX.ld;
         p.M = M;
         p.N = K;
         p.batch = 1;
-        if ((e = run_product<ET, false>(p, cx, ws, (int)(2 * Np), stream)) != hipSuccess) return e;
+        if ((e = run_product<ET, false, ALONG_K, ACROSS_K>(p, cx, ws, (int)(2 * half), stream)) != hipSuccess) return e;
     }
-    if (want_w) {
-        if ((e = transpose(X.ptr, X.ld, M, K, buf + at_xt, Mp, Mp, stream)) != hipSuccess) return e;
-        p.A[0] = buf + at_cols;
-        p.A[1] = buf + at_cols + (size_t)N * Mp * 2;
-        p.B[0] = p.B[1] = buf + at_xt;
-        p.lda = p.ldb[0] = p.ldb[1] = p.k_bytes = Mp * 2;
-        p.a_bytes = N * p.lda;
-        p.b_bytes[0] = p.b_bytes[1] = K * p.lda;
+    if (want_w) {  // dG^T X and dU^T X: the depth runs through the tokens
+        for (int z = 0; z < 2; ++z) {
+            p.A[z] = grads + z * half * 2;
+            p.B[z] = ptr[0];
+            p.ldb[z] = ld[0];
+            p.b_bytes[z] = (M - 1) * ld[0] + (int64_t)K * 2;
+        }
+        p.a_bytes = M * row - half * 2;
+        p.k_bytes = (int64_t)M * 2;
+        p.part_steps = 0x7fffffff;
         p.C[0] = dWg.ptr;
         p.C[1] = dWu.ptr;
         p.ldc[0] = dWg.ld;
@@ -401,7 +462,7 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         p.M = N;
         p.N = K;
         p.batch = 2;
-        if ((e = run_product<ET, false>(p, cw, ws, M, stream)) != hipSuccess) return e;
+        if ((e = run_product<ET, false, ACROSS_K, ACROSS_K>(p, cw, ws, M, stream)) != hipSuccess) return e;
     }
     return hipSuccess;
 }

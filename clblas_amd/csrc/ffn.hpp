@@ -18,7 +18,8 @@ struct Product {
     const void *B[2];       // gate's and other weight
     int64_t lda, ldb[2];
     int64_t a_bytes, b_bytes[2];  // from the first element to behind the last one
-    int64_t k_bytes;        // depth
+    int64_t k_bytes;        // depth (two bytes per index also where an operand's rows run across it)
+    int part_steps;         // steps of depth after which B[1] takes B[0]'s place (GATED has both at once: unused)
     const float *scale_a;   // 8-bit operands: one scale per row of A / B
     const float *scale_b[2];
     void *C[2];             // [batch entry]
@@ -29,7 +30,7 @@ struct Product {
     int batch;              // 1, or 2: two products A[z] B^T -> C[z]
     int out_type, gate;
     int tiles_m, tiles_n, group_m;
-    int splits, steps_per_split;  // depth ranges, and their length in steps of 128 bytes
+    int splits, steps_per_split;  // depth ranges, and their length in steps of 64 bytes (an even number)
     uint32_t *ws;           // partial sums of a split product
     int64_t ws_ld, ws_plane, ws_split;
 };

@@ -22,9 +22,7 @@ namespace ffn {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -34,24 +32,29 @@ template <> struct ElemOf<ET_I8> { typedef int8_t type; typedef int Acc; };
 template <> struct ElemOf<ET_F16> { typedef _Float16 type; typedef float Acc; };
 template <> struct ElemOf<ET_BF16> { typedef __bf16 type; typedef float Acc; };
 
-// One MFMA on MB x MB blocks.  Lane l holds row l % MB of either operand, the 16 bytes that start at byte
-// 16 (l / MB) of the instruction's depth (MB = 16: 64 bytes deep, MB = 32: 32 bytes).  Of the result it holds column
-// l % MB and, for every group q of four elements, rows 4 (64 / MB q + l / MB) .. + 3.
-template <int ET, int MB> struct Mfma;
-#define CBA_FFN_MFMA(ET, MB, ACC, OPND, BUILTIN)                                                              \
-    template <> struct Mfma<ET, MB> {                                                                         \
+// One MFMA on 16 x 16 blocks, 64 bytes deep.  Lane l holds row l % 16 of either operand, the 16 bytes from byte
+// 16 (l / 16) of the depth on; of the result it holds column l % 16, rows 4 (l / 16) .. + 3.
+template <int ET> struct Mfma;
+#define CBA_FFN_MFMA(ET, ACC, OPND, BUILTIN)                                                              \
+    template <> struct Mfma<ET> {                                                                         \
         typedef ACC Acc;                                                                                      \
         static __device__ __forceinline__ Acc run(u32x4 a, u32x4 b, Acc c) {                                  \
             return BUILTIN(__builtin_bit_cast(OPND, a), __builtin_bit_cast(OPND, b), c, 0, 0, 0);             \
         }                                                                                                     \
     };
-CBA_FFN_MFMA(ET_I8, 16, i32x4, i32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8)
-CBA_FFN_MFMA(ET_F16, 16, f32x4, f16x8, __builtin_amdgcn_mfma_f32_16x16x32_f16)
-CBA_FFN_MFMA(ET_BF16, 16, f32x4, bf16x8, __builtin_amdgcn_mfma_f32_16x16x32_bf16)
-CBA_FFN_MFMA(ET_I8, 32, i32x16, i32x4, __builtin_amdgcn_mfma_i32_32x32x32_i8)
-CBA_FFN_MFMA(ET_F16, 32, f32x16, f16x8, __builtin_amdgcn_mfma_f32_32x32x16_f16)
-CBA_FFN_MFMA(ET_BF16, 32, f32x16, bf16x8, __builtin_amdgcn_mfma_f32_32x32x16_bf16)
+CBA_FFN_MFMA(ET_I8, i32x4, i32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8)
+CBA_FFN_MFMA(ET_F16, f32x4, f16x8, __builtin_amdgcn_mfma_f32_16x16x32_f16)
+CBA_FFN_MFMA(ET_BF16, f32x4, bf16x8, __builtin_amdgcn_mfma_f32_16x16x32_bf16)
 #undef CBA_FFN_MFMA
+
+// A kernel's Product where the launch left it.  What is needed once per tile is read from there when it is needed, through a
+// pointer that the compiler cannot see through: it would keep some sixty scalar registers alive across the inner loop.
+typedef const __attribute__((address_space(4))) Product Args;
+static __device__ __forceinline__ Args *kernel_args() { return (Args *)__builtin_amdgcn_kernarg_segment_ptr(); }
+static __device__ __forceinline__ Args &fresh(Args *p) {
+    asm volatile("" : "+s"(p));
+    return *p;
+}
 
 // ---- elements of the result ----
 
@@ -118,7 +121,7 @@ static __device__ __forceinline__ void store4(int ot, void *base, int64_t at, co
 
 // Four neighbouring results (m, n .. n + 3) from their accumulators; `first` is the plain product or the gate's.
 template <int ET, bool GATED>
-static __device__ __forceinline__ void finish4(const Product &p, int z, int m, int n, const float *first, const float *second) {
+static __device__ __forceinline__ void finish4(Args &p, int z, int m, int n, const float *first, const float *second) {
     float x[4], u[4];
     const int valid = p.N - n;
     float sa = 1.f;
@@ -160,154 +163,547 @@ static __device__ __forceinline__ int xcd_contiguous(int id, int total) {
 
 // ---- the tiled product ----
 //
-// A workgroup computes a BM x BN tile of accumulators with waves of WM x WN.  Both operands travel HBM -> LDS without
-// passing through registers (buffer_load ... lds, 16 bytes per lane), 128 bytes of depth at a time, as rows of eight
-// 16-byte slots; slot s of row r is kept in place s ^ (r % 8), so that the eight rows that one pass of a fragment read
-// touches lie in different banks.  GATED: the BN rows are BN / 2 channels of either weight, arranged per wave (WN / 2
-// of the gate's, then the same WN / 2 channels of the other's), so that both factors of a result sit in the same lane.
-template <int ET_, int MB_, int BM_, int BN_, int WM_, int WN_, bool GATED_> struct TileCfg {
-    static constexpr int ET = ET_, MB = MB_, BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+// A workgroup computes BM x BN tiles of accumulators with waves of WM x WN.  Both operands travel HBM -> LDS without
+// passing through registers (buffer_load ... lds, 16 bytes per lane), one step of 64 bytes (32 or 64 elements, one MFMA
+// deep) at a time, through a ring of S stages.  Workgroups stay: each walks its part of the list of tiles, and the ring
+// runs on across the borders, so that the next tile's first steps are on their way while results are stored.
+//
+// An operand lies in memory either with its rows along the depth (ALONG_K: the forward products) or across it
+// (ACROSS_K, 16-bit types: a row per depth index, as the gradients meet weights and activations).
+//   ALONG_K   LDS image: a row of four 16-byte slots per tile row, slot s of row r in place s ^ (r / 2 % 4), so that the
+//             eight rows that one pass of a fragment read touches lie in different banks.
+//   ACROSS_K  LDS image: 32 rows of depth, each the tile's edge long.  A lane reads V neighbouring columns (8 or 4 bytes) of
+//             its 8 rows of depth and swaps 16-bit halves between row pairs (v_perm_b32): that gives it the operands
+//             of V MFMA blocks, block e holding columns e, V + e, 2 V + e ...  (The transposing LDS reads would do
+//             this without the swaps, but the compiler makes each of them wait for every load into LDS that is in
+//             flight: 2048 x 4096 x 4096, both operands across, 231 us.)
+// GATED: the BN rows of weights are BN / 2 channels of either weight, arranged per wave (WN / 2 of the gate's, then the
+// same WN / 2 channels of the other's), so that both factors of a result end up in the same lane.
+enum Lay { ALONG_K = 0, ACROSS_K = 1 };
+
+template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay LAYA_ = ALONG_K, Lay LAYB_ = ALONG_K> struct TileCfg {
+    static constexpr int ET = ET_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
     static constexpr bool GATED = GATED_;
+    static constexpr Lay LAYA = LAYA_, LAYB = LAYB_;
     static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
     static constexpr int CHANNELS = GATED ? BN / 2 : BN;  // columns of the result per tile
-    static constexpr int TM = WM / MB, TN = WN / MB;
-    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // wave-wide loads per step (8 rows each)
-    static constexpr int STAGE = (BM + BN) * 128;
-    static constexpr int LDS = 2 * STAGE;
-    static constexpr int KSTEPS = MB == 16 ? 2 : 4;  // MFMAs that take up 128 bytes of depth
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "rows divide over the waves");
-    static_assert(!GATED || (WN / 2) % MB == 0, "the halves of a wave's columns are whole blocks");
-    static_assert(!GATED || (WN / 2) % 8 == 0, "one load stays inside one weight");
+    // B in two parts, one after the other along the depth (the gradient of the input: both weights)
+    static constexpr bool PARTS = LAYA == ALONG_K && LAYB == ACROSS_K;
+    static constexpr int TM = WM / 16, TN = WN / 16;
+    static constexpr int LA = BM / 16 / WAVES, LB = BN / 16 / WAVES;  // wave-wide loads per step (1 KiB each)
+    static constexpr int STAGE = (BM + BN) * 64;
+    static constexpr int LDS = S * STAGE;
+    static_assert(BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0, "rows divide over the waves");
+    static_assert(!GATED || (WN / 2) % 16 == 0, "the halves of a wave's columns are whole blocks, and whole loads");
+    static_assert(!GATED || LAYB == ALONG_K, "");
+    static_assert(ET != ET_I8 || (LAYA == ALONG_K && LAYB == ALONG_K), "half swaps are for 16-bit types");
+    static_assert(LDS <= 160 * 1024 && S >= 2 && (S - 1) * (LA + LB) < 64, "");
 };
 
-template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 1) void tile_kernel(Product p) {
-    extern __shared__ __attribute__((aligned(128))) char lds[];
-    constexpr int MB = Cfg::MB, BM = Cfg::BM;
-    typedef Mfma<Cfg::ET, MB> Op;
+// How one wave-wide load fills its 1 KiB of an operand's LDS image.  X: tile edge.
+template <int X, Lay LAY> struct Image {
+    static constexpr int PER_ROW = LAY == ALONG_K ? 4 : X / 8;  // 16-byte slots
+    static constexpr int ROW = PER_ROW * 16;                    // bytes
+    static constexpr int ROWS_PER_LOAD = 64 / PER_ROW;
+    static __device__ __forceinline__ int swizzle(int row) {
+        if (LAY == ALONG_K) return (row >> 1) & 3;
+        return PER_ROW >= 16 ? ((row >> 3) & 1) << 3 : 0;  // (lane groups of a read are eight rows apart)
+    }
+    // Row and 16-byte slot (of memory) that this lane fetches in wave-wide load `q`.
+    static __device__ __forceinline__ int row_of(int q, int lane) { return q * ROWS_PER_LOAD + lane / PER_ROW; }
+    static __device__ __forceinline__ int slot_of(int q, int lane) { return (lane % PER_ROW) ^ swizzle(row_of(q, lane)); }
+};
+
+// MFMA operands of NBLK blocks of 16 rows, from tile row x0 of the image on.  read() fetches as many registers as one
+// block takes; ready() turns the V blocks of a group, read in raw form, into operands.
+template <int X, Lay LAY, int NBLK> struct Fragments {
+    typedef Image<X, LAY> Im;
+    static constexpr int V = LAY == ALONG_K ? 1 : NBLK % 4 == 0 ? 4 : 2;  // blocks per group
+    static_assert(NBLK % V == 0, "");
+    int off[NBLK / V];
+    __device__ __forceinline__ void init(int lane, int x0) {
+        const int r = lane & 15, g = lane >> 4;
+        if constexpr (LAY == ALONG_K) {
+            off[0] = (x0 + r) * Im::ROW + ((g ^ ((r >> 1) & 3)) << 4);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NBLK / V; ++u) {
+                const int at = (x0 + u * 16 * V + V * r) * 2;
+                off[u] = 8 * g * Im::ROW + (((at >> 4) ^ Im::swizzle(8 * g)) << 4) + (at & 15);
+            }
+        }
+    }
+    __device__ __forceinline__ u32x4 read(const char *base, int j) const {
+        if constexpr (LAY == ALONG_K) {
+            return *reinterpret_cast<const u32x4 *>(base + off[0] + j * 16 * Im::ROW);
+        } else if constexpr (V == 4) {
+            const char *at = base + off[j / 4] + 2 * (j % 4) * Im::ROW;
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(at), y = *reinterpret_cast<const u32x2 *>(at + Im::ROW);
+            return u32x4{x[0], x[1], y[0], y[1]};
+        } else {
+            const char *at = base + off[j / 2] + 4 * (j % 2) * Im::ROW;
+            return u32x4{*reinterpret_cast<const uint32_t *>(at), *reinterpret_cast<const uint32_t *>(at + Im::ROW),
+                         *reinterpret_cast<const uint32_t *>(at + 2 * Im::ROW), *reinterpret_cast<const uint32_t *>(at + 3 * Im::ROW)};
+        }
+    }
+    static __device__ __forceinline__ uint32_t halves(uint32_t row, uint32_t next_row, int e) {
+        return __builtin_amdgcn_perm(next_row, row, e & 1 ? 0x07060302u : 0x05040100u);
+    }
+    // f: the V registers quadruples of one group
+    static __device__ __forceinline__ void ready(u32x4 *f) {
+        if constexpr (V == 4) {
+            u32x4 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[e][q] = halves(f[q][e >> 1], f[q][2 + (e >> 1)], e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = o[e];
+        } else if constexpr (V == 2) {
+            u32x4 o[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[e][q] = halves(f[q >> 1][2 * (q & 1)], f[q >> 1][2 * (q & 1) + 1], e);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) f[e] = o[e];
+        }
+    }
+    // Row (within the wave's) that lane place r of block j stands for.
+    static __device__ __forceinline__ int row(int j, int r) { return V == 1 ? 16 * j + r : j / V * (16 * V) + V * r + j % V; }
+};
+
+// s_waitcnt immediates (gfx9: vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
+#define CBA_FFN_WAIT_VM(n) __builtin_amdgcn_s_waitcnt((((n) & 0xf) | (((n) >> 4) << 14) | (0x7 << 4) | (0xf << 8)))
+#define CBA_FFN_WAIT_LDS() __builtin_amdgcn_s_waitcnt((0xf | (3 << 14) | (0x7 << 4)))
+
+// Where entry `id` of the list of tiles, batch entries and depth ranges lies.
+struct TileAt {
+    int m0, n0, z, split, first_step, steps;  // steps: even, the last may be empty
+    int64_t depth;                            // bytes from first_step on
+};
+template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p, int id) {
+    TileAt t;
+    const int tiles = p.tiles_m * p.tiles_n;
+    t.split = id / (tiles * p.batch);
+    id -= t.split * tiles * p.batch;
+    t.z = id / tiles;
+    id -= t.z * tiles;
+    // groups of group_m tile rows, column by column: tiles that run together share both operands' rows in an L2
+    const int per_group = p.group_m * p.tiles_n, grp = id / per_group, first_m = grp * p.group_m;
+    const int gm = p.tiles_m - first_m < p.group_m ? p.tiles_m - first_m : p.group_m;
+    const int in_group = id - grp * per_group;
+    t.m0 = (first_m + in_group % gm) * Cfg::BM;
+    t.n0 = in_group / gm * Cfg::CHANNELS;
+    t.first_step = t.split * p.steps_per_split;
+    t.depth = p.k_bytes - (int64_t)t.first_step * 64;
+    const int64_t all = (t.depth + 127) >> 7 << 1;
+    t.steps = all < p.steps_per_split ? (int)all : p.steps_per_split;
+    return t;
+}
+
+// Tiles id, id + stride, ... below `end`.
+template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *args, int id, int stride, int end, char *lds) {
+    constexpr int BM = Cfg::BM, BN = Cfg::BN, TM = Cfg::TM, TN = Cfg::TN, S = Cfg::S, LA = Cfg::LA, LB = Cfg::LB;
+    typedef Mfma<Cfg::ET> Op;
     typedef typename Op::Acc Acc;
+    typedef Image<BM, Cfg::LAYA> ImA;
+    typedef Image<BN, Cfg::LAYB> ImB;
+    typedef Fragments<BM, Cfg::LAYA, TM> FragA;
+    typedef Fragments<BN, Cfg::LAYB, TN> FragB;
+    if (id >= end) return;
+    Args &p = *args;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / Cfg::WAVES_N, wn = wave % Cfg::WAVES_N;
 
-    // tile, split and batch entry of this workgroup
-    const int tiles = p.tiles_m * p.tiles_n;
-    int id = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int split = id / (tiles * p.batch);
-    id -= split * tiles * p.batch;
-    const int z = id / tiles;
-    id -= z * tiles;
-    const int per_group = p.group_m * p.tiles_n, grp = id / per_group, first_m = grp * p.group_m;
-    const int gm = p.tiles_m - first_m < p.group_m ? p.tiles_m - first_m : p.group_m;
-    const int r_in = id - grp * per_group;
-    const int m0 = (first_m + r_in % gm) * BM, n0 = r_in / gm * Cfg::CHANNELS;
+    // The lane's place in what it loads.  (The swizzle repeats after as many rows as lie between two loads of a wave.)
+    static_assert(Cfg::LAYA == ALONG_K || Cfg::WAVES * ImA::ROWS_PER_LOAD % 16 == 0, "");
+    static_assert(Cfg::LAYB == ALONG_K || Cfg::WAVES * ImB::ROWS_PER_LOAD % 16 == 0, "");
+    const int a_slot = ImA::slot_of(wave, lane) * 16, b_slot = ImB::slot_of(wave, lane) * 16;
+    const int lda = (int)p.lda, ldb[2] = {(int)p.ldb[0], (int)p.ldb[1]};
+    const int a_off = ImA::row_of(0, lane) * lda + a_slot;
+    const int b_off[2] = {ImB::row_of(0, lane) * ldb[0] + b_slot, ImB::row_of(0, lane) * ldb[1] + b_slot};
+    const int64_t a_step = Cfg::LAYA == ALONG_K ? 64 : 32 * p.lda;
+    const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 64 : 32 * p.ldb[0], Cfg::LAYB == ALONG_K ? 64 : 32 * p.ldb[1]};
+    const char *b_ptr[2] = {static_cast<const char *>(p.B[0]), static_cast<const char *>(p.B[1])};
+    const int64_t b_len[2] = {p.b_bytes[0], p.b_bytes[1]};
+    constexpr int kOutside = (int)0x80000000u;
 
-    const int64_t k0 = (int64_t)split * p.steps_per_split * 128;  // bytes
-    const int64_t k_left = p.k_bytes - k0;
-    const int steps_all = (int)((k_left + 127) >> 7);
-    const int steps = steps_all < p.steps_per_split ? steps_all : p.steps_per_split;
-
-    // Operands from this tile's first element on, and this lane's place in the rows it loads.
-    const char *a_base = static_cast<const char *>(p.A[z]) + (int64_t)m0 * p.lda + k0;
-    int64_t a_left = p.a_bytes - (int64_t)m0 * p.lda - k0;
-    const char *b_base[2];
-    int64_t b_left[2];
-#pragma unroll
-    for (int h = 0; h < (Cfg::GATED ? 2 : 1); ++h) {
-        b_base[h] = static_cast<const char *>(p.B[h]) + (int64_t)n0 * p.ldb[h] + k0;
-        b_left[h] = p.b_bytes[h] - (int64_t)n0 * p.ldb[h] - k0;
-    }
-    const int row8 = lane >> 3, slot = (lane & 7) ^ row8;
-    // (in the last step the slots beyond the depth are sent out of range and read as zero)
-    const int last_slots = (int)((k_left - (int64_t)(steps - 1) * 128) >> 4);
-    constexpr uint32_t kOutside = 0x80000000u;
-
-    auto issue = [&](int step, int stage) {
-        char *dst = lds + stage * Cfg::STAGE;
-        const bool out = step == steps - 1 && slot >= last_slots;
-        const int64_t at = (int64_t)step * 128;
-        const __amdgpu_buffer_rsrc_t ra = rsrc_of(a_base + at, a_left - at);
-#pragma unroll
-        for (int i = 0; i < Cfg::LA; ++i) {
-            const int row = (wave + i * Cfg::WAVES) * 8;
-            const uint32_t off = (uint32_t)((row + row8) * (int)p.lda + slot * 16);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t *)(dst + row * 128), 16, (int)(out ? kOutside : off), 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < Cfg::LB; ++i) {
-            const int row = (wave + i * Cfg::WAVES) * 8;
-            const int h = Cfg::GATED ? (row % Cfg::WN) / (Cfg::WN / 2) : 0;
-            const int ch = Cfg::GATED ? row / Cfg::WN * (Cfg::WN / 2) + row % (Cfg::WN / 2) : row;
-            const __amdgpu_buffer_rsrc_t rb = rsrc_of((h ? b_base[1] : b_base[0]) + at, (h ? b_left[1] : b_left[0]) - at);
-            const uint32_t off = (uint32_t)((ch + row8) * (int)(h ? p.ldb[1] : p.ldb[0]) + slot * 16);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void_t *)(dst + (BM + row) * 128), 16, (int)(out ? kOutside : off), 0, 0, 0);
+    // The feeding side runs S steps ahead of the multiplying one.  feed_*: operands from the next step on.
+    TileAt feed = tile_at<Cfg>(fresh(args), id);
+    int feed_id = id, feed_step = 0, part = 0;
+    const char *feed_a, *feed_b[2];
+    int64_t left_a, left_b[2];
+    auto aim_b = [&](int h, int step) {  // at a step within B[h]
+        Args &p = fresh(args);
+        const int64_t skip = (Cfg::LAYB == ALONG_K ? feed.n0 * p.ldb[h] : (int64_t)feed.n0 * 2) + step * b_step[h];
+        const int to = Cfg::GATED ? h : 0;
+        feed_b[to] = static_cast<const char *>(p.B[h]) + skip;
+        left_b[to] = p.b_bytes[h] - skip;
+    };
+    // (PARTS: aimed anew for every step, without a branch)
+    const int part_steps = Cfg::PARTS ? p.part_steps : 0;
+    auto aim_parts = [&] {
+        const int step = feed.first_step + feed_step;
+        part = step >= part_steps;
+        const int64_t skip = (int64_t)feed.n0 * 2 + (int64_t)(part ? step - part_steps : step) * (part ? b_step[1] : b_step[0]);
+        feed_b[0] = (part ? b_ptr[1] : b_ptr[0]) + skip;
+        left_b[0] = (part ? b_len[1] : b_len[0]) - skip;
+    };
+    auto aim = [&] {
+        Args &p = fresh(args);
+        const int64_t skip = (Cfg::LAYA == ALONG_K ? feed.m0 * p.lda : (int64_t)feed.m0 * 2) + feed.first_step * a_step;
+        feed_a = static_cast<const char *>(p.A[feed.z]) + skip;
+        left_a = p.a_bytes - skip;
+        if constexpr (Cfg::PARTS) {
+            aim_parts();
+        } else {
+            aim_b(0, feed.first_step);
+            if (Cfg::GATED) aim_b(1, feed.first_step);
         }
     };
+    aim();
+    // Starts one of the LA + LB loads of the feeding side's step.  ALONG_K: slots behind the depth's end, and everything
+    // once the last tile has been fed, go out of range, where loads give zeros.  (ACROSS_K: rows behind it lie behind the
+    // operand's last byte.)
+    auto issue_one = [&](char *dst, int i) {
+        const int64_t left = feed_id < end ? feed.depth - (int64_t)feed_step * 64 : 0;
+        const int depth = left < 64 ? (int)left : 64;
+        if (i < LA) {
+            const int q = wave + i * Cfg::WAVES;
+            const bool out = Cfg::LAYA == ALONG_K ? a_slot >= depth : feed_id >= end;
+            const int off = a_off + q * ImA::ROWS_PER_LOAD * lda;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(feed_a, left_a), (lds_void_t *)(dst + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
+        } else {
+            const int q = wave + (i - LA) * Cfg::WAVES;
+            const int row = q * ImB::ROWS_PER_LOAD;
+            const int h = Cfg::GATED ? (row % Cfg::WN) / (Cfg::WN / 2) : 0;
+            const int ch = Cfg::GATED ? row / Cfg::WN * (Cfg::WN / 2) + row % (Cfg::WN / 2) : row;
+            const bool out = Cfg::LAYB == ALONG_K ? b_slot >= depth : feed_id >= end;
+            const bool second = Cfg::GATED ? h : Cfg::PARTS ? part : 0;
+            const int off = (second ? b_off[1] : b_off[0]) + ch * (second ? ldb[1] : ldb[0]);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(h ? feed_b[1] : feed_b[0], h ? left_b[1] : left_b[0]),
+                                                     (lds_void_t *)(dst + BM * 64 + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
+        }
+    };
+    auto feed_on = [&] {
+        ++feed_step;
+        if (feed_step == feed.steps) {
+            feed_id += stride;
+            feed_step = 0;
+            if (feed_id < end) {
+                feed = tile_at<Cfg>(fresh(args), feed_id);
+                aim();
+            }
+            return;
+        }
+        feed_a += a_step;
+        left_a -= a_step;
+        if constexpr (Cfg::PARTS) {
+            aim_parts();
+        } else {
+#pragma unroll
+            for (int h = 0; h < (Cfg::GATED ? 2 : 1); ++h) {
+                feed_b[h] += b_step[h];
+                left_b[h] -= b_step[h];
+            }
+        }
+    };
+    // A slot that the depth ends in (its last bytes are real memory: the next row) is cut off in LDS once it is there - for
+    // both operands, as zero times NaN is no zero.
+    auto cut = [&](char *dst, int q, int slot, int depth) {
+        if (slot != (depth & ~15)) return;
+        u32x4 *at = reinterpret_cast<u32x4 *>(dst + q * 1024 + lane * 16);
+        u32x4 v = *at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int keep = (depth & 15) - 4 * e;  // bytes of this dword
+            v[e] = keep >= 4 ? v[e] : keep <= 0 ? 0u : v[e] & ((1u << (8 * keep)) - 1);
+        }
+        *at = v;
+    };
+    // What this wave loaded of a step is in LDS: make it fit to be read, then wait for the other waves.  depth: from that
+    // step on.
+    auto publish = [&](char *dst, int64_t depth) {
+        if (depth < 64 && depth > 0 && (depth & 15)) {
+            if (Cfg::LAYA == ALONG_K)
+#pragma unroll
+                for (int i = 0; i < LA; ++i) cut(dst, wave + i * Cfg::WAVES, a_slot, (int)depth);
+            if (Cfg::LAYB == ALONG_K)
+#pragma unroll
+                for (int i = 0; i < LB; ++i) cut(dst + BM * 64, wave + i * Cfg::WAVES, b_slot, (int)depth);
+        }
+        CBA_FFN_WAIT_LDS();  // also: this wave's fragment reads of the stage that is loaded into next have completed
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
 
-    Acc acc[Cfg::TM][Cfg::TN];
-#pragma unroll
-    for (int i = 0; i < Cfg::TM; ++i)
-#pragma unroll
-        for (int j = 0; j < Cfg::TN; ++j) acc[i][j] = Acc{};
+    FragA ra;
+    FragB rb;
+    ra.init(lane, wm * Cfg::WM);
+    rb.init(lane, wn * Cfg::WN);
+    u32x4 fa[2][TM], fb[2][TN];  // operands of this step and the next
+    auto read_one = [&](const char *stage, int set, int i) {
+        if (i < TN) fb[set][i] = rb.read(stage + BM * 64, i);
+        else fa[set][i - TN] = ra.read(stage, i - TN);
+    };
+    Acc acc[TM][TN];
 
-    const int r = lane % MB, g = lane / MB;
-    const int frag0 = r * 128 + ((g ^ (r & 7)) << 4);
-    if (steps > 0) issue(0, 0);
-    for (int s = 0; s < steps; ++s) {
-        __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
-        __syncthreads();
-        if (s + 1 < steps) issue(s + 1, (s + 1) & 1);
-        const char *as = lds + (s & 1) * Cfg::STAGE + wm * Cfg::WM * 128;
-        const char *bs = lds + (s & 1) * Cfg::STAGE + (BM + wn * Cfg::WN) * 128;
+    char *stage = lds;
+    auto after = [&](char *st) { return st + Cfg::STAGE == lds + Cfg::LDS ? lds : st + Cfg::STAGE; };
+#pragma nounroll
+    for (int s = 0; s < S; ++s) {
 #pragma unroll
-        for (int kk = 0; kk < Cfg::KSTEPS; ++kk) {
-            const int off = frag0 ^ (kk * (128 / Cfg::KSTEPS));
-            u32x4 a[Cfg::TM], b[Cfg::TN];
+        for (int i = 0; i < LA + LB; ++i) issue_one(lds + s * Cfg::STAGE, i);
+        feed_on();
+    }
+    TileAt t = tile_at<Cfg>(fresh(args), id);
+    CBA_FFN_WAIT_VM((S - 1) * (LA + LB));
+    publish(lds, t.depth);
 #pragma unroll
-            for (int i = 0; i < Cfg::TM; ++i) a[i] = *reinterpret_cast<const u32x4 *>(as + i * MB * 128 + off);
+    for (int i = 0; i < TM + TN; ++i) read_one(lds, 0, i);
+
+    // One step: publish the next one, then multiply this one's operands while the next one's are read and the loads of the
+    // step S later start into the stage that has become free.
+    auto step = [&](int set, int64_t next_depth) {
+        char *next = after(stage);
+        CBA_FFN_WAIT_VM((S - 2) * (LA + LB));
+        publish(next, next_depth);
+        constexpr int OTHER = TM + TN > LA + LB ? TM + TN : LA + LB;
 #pragma unroll
-            for (int j = 0; j < Cfg::TN; ++j) b[j] = *reinterpret_cast<const u32x4 *>(bs + j * MB * 128 + off);
+        for (int j = 0; j < TN; j += FragB::V) rb.ready(&fb[set][j]);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int o = OTHER * i / TM; o < OTHER * (i + 1) / TM; ++o) {
+                if (o < LA + LB) issue_one(stage, o);
+                if (o < TM + TN) read_one(next, set ^ 1, o);
+            }
+            if (i % FragA::V == 0) ra.ready(&fa[set][i]);
             // the weights are the instruction's first operand: a lane then holds one token's neighbouring channels
 #pragma unroll
-            for (int i = 0; i < Cfg::TM; ++i)
+            for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[set][j], fa[set][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        feed_on();
+        stage = next;
+    };
+
+    const int r = lane & 15, g = lane >> 4;
+    for (;;) {
 #pragma unroll
-                for (int j = 0; j < Cfg::TN; ++j) acc[i][j] = Op::run(b[j], a[i], acc[i][j]);
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
+        const int next_id = id + stride;
+        const int64_t next_tile_depth = next_id < end ? tile_at<Cfg>(fresh(args), next_id).depth : 0;
+        int64_t depth = t.depth;
+        for (int s = 0; s < t.steps; s += 2) {
+            step(0, depth - 64);
+            depth -= 128;
+            step(1, s + 2 < t.steps ? depth : next_tile_depth);
+        }
+
+        Args &out = fresh(args);
+        // results: four neighbouring columns of a row at a time
+        constexpr int HALF = Cfg::GATED ? TN / 2 : TN, J2 = Cfg::GATED ? HALF : 0;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int m = t.m0 + wm * Cfg::WM + FragA::row(i, r);
+            if (m >= out.M) continue;
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) {
+                // ALONG_K: the four elements of accumulator j; else element e comes from the e-th block of a group
+                constexpr int V = FragB::V;
+                const int n = t.n0 + wn * (HALF * 16) + (V == 1 ? 16 * j + 4 * g : V == 4 ? j / 4 * 64 + 16 * g + 4 * (j % 4) : j / 2 * 32 + 8 * g + 4 * (j % 2));
+                if (n >= out.N) continue;
+                Acc x, u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = V == 1 ? acc[i][j][e] : V == 4 ? acc[i][j / 4 * 4 + e][j % 4] : acc[i][j / 2 * 2 + (e & 1)][2 * (j % 2) + (e >> 1)];
+                    u[e] = acc[i][j + J2][e];
+                }
+                if (out.splits > 1) {
+                    typedef typename ElemOf<Cfg::ET>::Acc Sum;
+                    Sum *w = reinterpret_cast<Sum *>(out.ws) + (int64_t)t.split * out.ws_split + (int64_t)t.z * out.ws_plane + (int64_t)m * out.ws_ld + n;
+                    *reinterpret_cast<Acc *>(w) = x;
+                    if (Cfg::GATED) *reinterpret_cast<Acc *>(w + out.ws_plane) = u;
+                } else {
+                    const float fx[4] = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+                    const float fu[4] = {(float)u[0], (float)u[1], (float)u[2], (float)u[3]};
+                    finish4<Cfg::ET, Cfg::GATED>(out, t.z, m, n, fx, fu);
+                }
+            }
+        }
+        if (next_id >= end) break;
+        id = next_id;
+        t = tile_at<Cfg>(fresh(args), id);
+    }
+    CBA_FFN_WAIT_VM(0);  // (nothing may be on its way into LDS when the workgroup ends)
+}
+
+// Workgroups are handed to the 8 XCDs in turn, and each XCD has an L2 of its own: every XCD walks a contiguous piece of the
+// list, its workgroups side by side.
+template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void tile_kernel(Product p) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int total = p.tiles_m * p.tiles_n * p.batch * p.splits;
+    const int xcds = gridDim.x < 8 ? gridDim.x : 8, xcd = blockIdx.x % xcds, place = blockIdx.x / xcds;
+    const int per = total / xcds, rem = total % xcds;
+    const int first = xcd * per + (xcd < rem ? xcd : rem), end = first + per + (xcd < rem ? 1 : 0);
+    const int stride = (gridDim.x - xcd + xcds - 1) / xcds;  // workgroups on this XCD
+    walk_tiles<Cfg>(kernel_args(), first + place, stride, end, lds);
+}
+
+// ---- the product from registers ----
+//
+// For products too small to fill the card with large tiles, or to pay for a round trip through LDS: a workgroup computes
+// a tile of 16 TM x 16 TN (GATED: 16 TN channels of both weights), and its W waves share the DEPTH, wave w taking every
+// W-th piece of 128 bytes.  So no wave needs what another has loaded: each reads its rows from memory straight into the
+// MFMAs' registers, DEEP pieces ahead, without a barrier, and the W partial tiles are added up in LDS once at the end
+// (in wave order).  Loads need no alignment; rows behind the last one are read as the last one, and not stored.
+template <int ET_, int TM_, int TN_, int W_, int DEEP_, bool GATED_> struct RowsCfg {
+    static constexpr int ET = ET_, TM = TM_, TN = TN_, W = W_, DEEP = DEEP_;
+    static constexpr bool GATED = GATED_;
+    static constexpr int NB = GATED ? 2 * TN : TN;  // blocks of weights' rows
+    static constexpr int THREADS = 64 * W;
+    static constexpr int PITCH = 16 * NB + 4;        // of a partial tile's row in LDS, 32-bit sums
+    static constexpr int LDS = W * 16 * TM * PITCH * 4;
+};
+
+// The 16 bytes of a row from byte `at` on, as far as they lie before `end` (zeros behind).
+template <int ES> static __device__ __forceinline__ u32x4 load16_tail(const char *row, int64_t at, int64_t end) {
+    u32x4 v = {};
+    if (at + 16 <= end) {
+        __builtin_memcpy(&v, row + at, 16);
+        return v;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e += ES)
+        if (at + e < end) {
+            uint32_t x;
+            if (ES == 2) {
+                uint16_t y;
+                __builtin_memcpy(&y, row + at + e, 2);
+                x = y;
+            } else {
+                x = *reinterpret_cast<const uint8_t *>(row + at + e);
+            }
+            v[e / 4] |= x << (8 * (e % 4));
+        }
+    return v;
+}
+
+template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void rows_kernel(Product p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int TM = Cfg::TM, TN = Cfg::TN, NB = Cfg::NB, W = Cfg::W, D = Cfg::DEEP, ES = Cfg::ET == ET_I8 ? 1 : 2;
+    typedef Mfma<Cfg::ET> Op;
+    typedef typename ElemOf<Cfg::ET>::Acc S;
+    typedef S sx4 __attribute__((ext_vector_type(4)));
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // neighbours in the list share the weights' rows, and an XCD gets a contiguous piece of it
+    const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int m0 = id % p.tiles_m * (16 * TM), n0 = id / p.tiles_m * (16 * TN);
+
+    const char *a[TM], *b[NB];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = m0 + 16 * i + r;
+        a[i] = static_cast<const char *>(p.A[0]) + (int64_t)(m < p.M ? m : p.M - 1) * p.lda;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int h = Cfg::GATED && j >= TN ? 1 : 0;
+        const int n = n0 + 16 * (j - h * TN) + r;
+        b[j] = static_cast<const char *>(p.B[h]) + (int64_t)(n < p.N ? n : p.N - 1) * p.ldb[h];
+    }
+    sx4 acc[TM][NB] = {};
+    u32x4 fa[D][TM][2], fb[D][NB][2];
+    auto load = [&](int d, int piece) {
+        const int64_t at = (int64_t)piece * 128 + g * 16;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) __builtin_memcpy(&fb[d][j][kk], b[j] + at + 64 * kk, 16);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) __builtin_memcpy(&fa[d][i][kk], a[i] + at + 64 * kk, 16);
+        }
+    };
+    auto use = [&](int d) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = Op::run(fb[d][j][kk], fa[d][i][kk], acc[i][j]);
+    };
+    // pieces wave, wave + W, ... of the whole ones are this wave's
+    const int whole = (int)(p.k_bytes >> 7), mine = whole > wave ? (whole - wave + W - 1) / W : 0;
+    int i0 = 0;
+    if (mine >= D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) load(d, wave + d * W);
+        for (; i0 + 2 * D <= mine; i0 += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                use(d);
+                load(d, wave + (i0 + D + d) * W);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) use(d);
+        i0 += D;
+    }
+    if (i0 < mine) {
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (i0 + d < mine) load(d, wave + (i0 + d) * W);
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (i0 + d < mine) use(d);
+    }
+    if ((p.k_bytes & 127) && whole % W == wave) {
+        const int64_t at = (int64_t)whole * 128 + g * 16;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            if (kk && (p.k_bytes & 127) <= 64) continue;
+            u32x4 ta[TM], tb[NB];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) ta[i] = load16_tail<ES>(a[i], at + 64 * kk, p.k_bytes);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) tb[j] = load16_tail<ES>(b[j], at + 64 * kk, p.k_bytes);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = Op::run(tb[j], ta[i], acc[i][j]);
         }
     }
 
-    constexpr int HALF = Cfg::GATED ? Cfg::TN / 2 : Cfg::TN, QUADS = MB * MB / 64 / 4;
+    // partial tiles [wave][m][n] -> sums -> results
+    S *part = reinterpret_cast<S *>(lds);
 #pragma unroll
-    for (int i = 0; i < Cfg::TM; ++i) {
-        const int m = m0 + wm * Cfg::WM + i * MB + r;
-        if (m >= p.M) continue;
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < HALF; ++j)
+        for (int j = 0; j < NB; ++j)
+            *reinterpret_cast<sx4 *>(part + ((wave * TM + i) * 16 + r) * Cfg::PITCH + 16 * j + 4 * g) = acc[i][j];
+    __syncthreads();
+    constexpr int QUADS = 16 * TM * 4 * TN;
 #pragma unroll
-            for (int q = 0; q < QUADS; ++q) {
-                const int n = n0 + wn * (HALF * MB) + j * MB + 4 * (64 / MB * q + g);
-                if (n >= p.N) continue;
-                constexpr int J2 = Cfg::GATED ? HALF : 0;
-                if (p.splits > 1) {
-                    typedef typename ElemOf<Cfg::ET>::Acc S;
-                    typedef S sx4 __attribute__((ext_vector_type(4)));
-                    S *w = reinterpret_cast<S *>(p.ws) + (int64_t)split * p.ws_split + (int64_t)z * p.ws_plane + (int64_t)m * p.ws_ld + n;
-                    sx4 v, v2;
+    for (int q0 = 0; q0 < QUADS; q0 += Cfg::THREADS) {
+        const int q = q0 + tid, ml = q / (4 * TN), nl = q % (4 * TN) * 4;
+        const int m = m0 + ml, n = n0 + nl;
+        if ((QUADS % Cfg::THREADS && q >= QUADS) || m >= p.M || n >= p.N) continue;
+        sx4 x = {}, y = {};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = acc[i][j][4 * q + e];
-                        v2[e] = acc[i][j + J2][4 * q + e];
-                    }
-                    *reinterpret_cast<sx4 *>(w) = v;
-                    if (Cfg::GATED) *reinterpret_cast<sx4 *>(w + p.ws_plane) = v2;
-                } else {
-                    float x[4], u[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = (float)acc[i][j][4 * q + e];
-                        u[e] = (float)acc[i][j + J2][4 * q + e];
-                    }
-                    finish4<Cfg::ET, Cfg::GATED>(p, z, m, n, x, u);
-                }
-            }
+        for (int w = 0; w < W; ++w) {
+            const S *at = part + (w * TM * 16 + ml) * Cfg::PITCH + nl;
+            x += *reinterpret_cast<const sx4 *>(at);
+            if (Cfg::GATED) y += *reinterpret_cast<const sx4 *>(at + 16 * TN);
+        }
+        const float fx[4] = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]}, fy[4] = {(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+        finish4<Cfg::ET, Cfg::GATED>(*kernel_args(), 0, m, n, fx, fy);
     }
 }
 
@@ -331,7 +727,7 @@ template <int ET, bool GATED> __global__ __launch_bounds__(256) void join_kernel
         }
         float x[4] = {(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
         float y[4] = {(float)b[0], (float)b[1], (float)b[2], (float)b[3]};
-        finish4<ET, GATED>(p, z, m, n, x, y);
+        finish4<ET, GATED>(*kernel_args(), z, m, n, x, y);
     }
 }
 

@@ -57,6 +57,8 @@ struct DebugKnobs {
     int trsm_wide = -1;    // CLBLAS_AMD_TRSM_WIDE (real types, substitution leaf): 0 / 1 forces 16 / 32 right-hand sides per workgroup
     int trsm_leaf = 0;     // CLBLAS_AMD_TRSM_LEAF (real types): 0 substitution over 16-row sub-blocks, 1 inverted 64 x 64 triangles
     int wide_ld = 0;       // CLBLAS_AMD_GEMM_WIDE_LD=1: the wide-ld kernels whatever the leading dimensions (tests)
+    int ffn_form = -1;     // CLBLAS_AMD_FFN_FORM (feed-forward products): index of the kernel form to use, -1: the rule's choice (tests)
+    int ffn_splits = 0;    // CLBLAS_AMD_FFN_SPLITS: depth ranges of their tiled forms, 0: the rule's choice (tests)
     int deep_panels = 1;   // CLBLAS_AMD_GEMM_DEEP: 0 never the deep-panel variant of a tile, 1 by the rule, 2 wherever built, more: from that depth of a K range
 };
 const DebugKnobs &knobs();
