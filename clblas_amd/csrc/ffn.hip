@@ -210,18 +210,18 @@ template <typename Cfg> hipError_t launch_tiles(const Product &p, int K, hipStre
 // The tiled forms: edges, and the index by which a form is known (the forms that run from registers come first).
 enum { ROWS_FORMS = 6 };
 struct TileShape { int bm, bn; };
-const TileShape kTiles[] = {{256, 256}, {256, 256}, {128, 128}, {128, 256}, {64, 128}, {128, 64}, {64, 64}, {256, 128}};
+const TileShape kTiles[] = {{256, 256}, {256, 128}, {128, 128}, {128, 128}, {64, 128}, {64, 128}, {64, 64}, {128, 256}};
 
 template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
     switch (tile) {
-    case 0: return f(TileCfg<ET, 256, 256, 128, 64, 5, GATED, LA, LB>());
-    case 1: return f(TileCfg<ET, 256, 256, 128, 64, 4, GATED, LA, LB>());
+    case 0: return f(TileCfg<ET, 256, 256, 128, 64, 2, GATED, LA, LB>());
+    case 1: return f(TileCfg<ET, 256, 128, 64, 64, 3, GATED, LA, LB>());
     case 2: return f(TileCfg<ET, 128, 128, 64, 64, 5, GATED, LA, LB>());
-    case 3: return f(TileCfg<ET, 128, 256, 64, 64, 6, GATED, LA, LB>());
-    case 4: return f(TileCfg<ET, 64, 128, 32, 64, 6, GATED, LA, LB>());
-    case 5: return f(TileCfg<ET, 128, 64, 64, 32, 6, GATED, LA, LB>());
-    case 6: return f(TileCfg<ET, 64, 64, 32, 32, 8, GATED, LA, LB>());
-    default: return f(TileCfg<ET, 256, 128, 64, 64, 6, GATED, LA, LB>());
+    case 3: return f(TileCfg<ET, 128, 128, 64, 64, 2, GATED, LA, LB>());
+    case 4: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED, LA, LB>());
+    case 5: return f(TileCfg<ET, 64, 128, 32, 64, 6, GATED, LA, LB>());
+    case 6: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED, LA, LB>());
+    default: return f(TileCfg<ET, 128, 256, 64, 64, 3, GATED, LA, LB>());
     }
 }
 
@@ -250,8 +250,8 @@ TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
     }
     if (knobs().ffn_splits) splits = knobs().ffn_splits < steps ? knobs().ffn_splits : steps;
     if (splits < 1) splits = 1;
-    c.steps_per_split = 2 * (int)ceil_div(steps, splits);
-    c.splits = (int)ceil_div(2 * steps, c.steps_per_split);
+    c.steps_per_split = (int)ceil_div(steps, splits);
+    c.splits = (int)ceil_div(steps, c.steps_per_split);
     if (c.splits > 1) {
         c.ws_ld = round_up(N, 4);
         c.ws_plane = c.ws_ld * M;
@@ -437,7 +437,7 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
             p.b_bytes[h] = (N - 1) * ld[1 + h] + (int64_t)K * 2;
         }
         p.k_bytes = row;
-        p.part_steps = (int)(half / 32);
+        p.part_steps = (int)(half / 64);
         p.C[0] = p.C[1] = dX.ptr;
         p.ldc[0] = p.ldc[1] = dX.ld;
         p.M = M;

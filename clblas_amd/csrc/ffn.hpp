@@ -30,7 +30,7 @@ struct Product {
     int batch;              // 1, or 2: two products A[z] B^T -> C[z]
     int out_type, gate;
     int tiles_m, tiles_n, group_m;
-    int splits, steps_per_split;  // depth ranges, and their length in steps of 64 bytes (an even number)
+    int splits, steps_per_split;  // depth ranges, and their length in steps of 128 bytes
     uint32_t *ws;           // partial sums of a split product
     int64_t ws_ld, ws_plane, ws_split;
 };

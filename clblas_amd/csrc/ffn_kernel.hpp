@@ -149,8 +149,11 @@ static __device__ __forceinline__ void finish4(Args &p, int z, int m, int n, con
 static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void *p, int64_t bytes_left) {
     // An access reaches at most 2 GiB from its descriptor's base (the host sees to the row strides); what lies
     // beyond the operand's last byte reads as zero.  The length is rounded up to whole dwords: a 16-bit operand may
-    // end in the middle of one.
-    const int64_t n = bytes_left <= 0 ? 0 : (bytes_left > 0x7ffffffcLL ? 0x7ffffffcLL : ((bytes_left + 3) & ~3LL));
+    // end in the middle of one.  (In 32-bit scalar steps: the compiler compares 64 bits on the vector unit.)
+    const int high = (int)(bytes_left >> 31);
+    uint32_t n = ((uint32_t)bytes_left + 3) & ~3u;
+    n = high > 0 ? 0x7ffffffcu : n;
+    n = high < 0 ? 0u : n;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)n, 0x00020000);
 }
 
@@ -164,15 +167,16 @@ static __device__ __forceinline__ int xcd_contiguous(int id, int total) {
 // ---- the tiled product ----
 //
 // A workgroup computes BM x BN tiles of accumulators with waves of WM x WN.  Both operands travel HBM -> LDS without
-// passing through registers (buffer_load ... lds, 16 bytes per lane), one step of 64 bytes (32 or 64 elements, one MFMA
-// deep) at a time, through a ring of S stages.  Workgroups stay: each walks its part of the list of tiles, and the ring
+// passing through registers (buffer_load ... lds, 16 bytes per lane), one step of 128 bytes (64 or 128 elements, two MFMAs
+// deep) at a time, through a ring of S stages.  (Steps of 64 bytes allow a finer ring, but fetch half cache lines: 8192 x
+// 12288 x 4096 gated in 1370-1450 us against 1320.)  Workgroups stay: each walks its part of the list of tiles, and the ring
 // runs on across the borders, so that the next tile's first steps are on their way while results are stored.
 //
 // An operand lies in memory either with its rows along the depth (ALONG_K: the forward products) or across it
 // (ACROSS_K, 16-bit types: a row per depth index, as the gradients meet weights and activations).
-//   ALONG_K   LDS image: a row of four 16-byte slots per tile row, slot s of row r in place s ^ (r / 2 % 4), so that the
+//   ALONG_K   LDS image: a row of eight 16-byte slots per tile row, slot s of row r in place s ^ (r % 8), so that the
 //             eight rows that one pass of a fragment read touches lie in different banks.
-//   ACROSS_K  LDS image: 32 rows of depth, each the tile's edge long.  A lane reads V neighbouring columns (8 or 4 bytes) of
+//   ACROSS_K  LDS image: 64 rows of depth, each the tile's edge long.  A lane reads V neighbouring columns (8 or 4 bytes) of
 //             its 8 rows of depth and swaps 16-bit halves between row pairs (v_perm_b32): that gives it the operands
 //             of V MFMA blocks, block e holding columns e, V + e, 2 V + e ...  (The transposing LDS reads would do
 //             this without the swaps, but the compiler makes each of them wait for every load into LDS that is in
@@ -190,10 +194,10 @@ template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay 
     // B in two parts, one after the other along the depth (the gradient of the input: both weights)
     static constexpr bool PARTS = LAYA == ALONG_K && LAYB == ACROSS_K;
     static constexpr int TM = WM / 16, TN = WN / 16;
-    static constexpr int LA = BM / 16 / WAVES, LB = BN / 16 / WAVES;  // wave-wide loads per step (1 KiB each)
-    static constexpr int STAGE = (BM + BN) * 64;
+    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // wave-wide loads per step (1 KiB each)
+    static constexpr int STAGE = (BM + BN) * 128;
     static constexpr int LDS = S * STAGE;
-    static_assert(BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0, "rows divide over the waves");
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "rows divide over the waves");
     static_assert(!GATED || (WN / 2) % 16 == 0, "the halves of a wave's columns are whole blocks, and whole loads");
     static_assert(!GATED || LAYB == ALONG_K, "");
     static_assert(ET != ET_I8 || (LAYA == ALONG_K && LAYB == ALONG_K), "half swaps are for 16-bit types");
@@ -202,11 +206,11 @@ template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay 
 
 // How one wave-wide load fills its 1 KiB of an operand's LDS image.  X: tile edge.
 template <int X, Lay LAY> struct Image {
-    static constexpr int PER_ROW = LAY == ALONG_K ? 4 : X / 8;  // 16-byte slots
+    static constexpr int PER_ROW = LAY == ALONG_K ? 8 : X / 8;  // 16-byte slots
     static constexpr int ROW = PER_ROW * 16;                    // bytes
     static constexpr int ROWS_PER_LOAD = 64 / PER_ROW;
     static __device__ __forceinline__ int swizzle(int row) {
-        if (LAY == ALONG_K) return (row >> 1) & 3;
+        if (LAY == ALONG_K) return row & 7;
         return PER_ROW >= 16 ? ((row >> 3) & 1) << 3 : 0;  // (lane groups of a read are eight rows apart)
     }
     // Row and 16-byte slot (of memory) that this lane fetches in wave-wide load `q`.
@@ -214,17 +218,18 @@ template <int X, Lay LAY> struct Image {
     static __device__ __forceinline__ int slot_of(int q, int lane) { return (lane % PER_ROW) ^ swizzle(row_of(q, lane)); }
 };
 
-// MFMA operands of NBLK blocks of 16 rows, from tile row x0 of the image on.  read() fetches as many registers as one
-// block takes; ready() turns the V blocks of a group, read in raw form, into operands.
+// MFMA operands of NBLK blocks of 16 rows, from tile row x0 of the image on, for either MFMA (kk) of a step.  read() fetches
+// as many registers as one block takes; ready() turns the V blocks of a group, read in raw form, into operands.
 template <int X, Lay LAY, int NBLK> struct Fragments {
     typedef Image<X, LAY> Im;
     static constexpr int V = LAY == ALONG_K ? 1 : NBLK % 4 == 0 ? 4 : 2;  // blocks per group
     static_assert(NBLK % V == 0, "");
-    int off[NBLK / V];
+    int off[LAY == ALONG_K ? 2 : NBLK / V];
     __device__ __forceinline__ void init(int lane, int x0) {
         const int r = lane & 15, g = lane >> 4;
         if constexpr (LAY == ALONG_K) {
-            off[0] = (x0 + r) * Im::ROW + ((g ^ ((r >> 1) & 3)) << 4);
+            off[0] = (x0 + r) * Im::ROW + ((g ^ (r & 7)) << 4);
+            off[1] = off[0] ^ 64;
         } else {
 #pragma unroll
             for (int u = 0; u < NBLK / V; ++u) {
@@ -233,15 +238,15 @@ template <int X, Lay LAY, int NBLK> struct Fragments {
             }
         }
     }
-    __device__ __forceinline__ u32x4 read(const char *base, int j) const {
+    __device__ __forceinline__ u32x4 read(const char *base, int j, int kk) const {
         if constexpr (LAY == ALONG_K) {
-            return *reinterpret_cast<const u32x4 *>(base + off[0] + j * 16 * Im::ROW);
+            return *reinterpret_cast<const u32x4 *>(base + off[kk] + j * 16 * Im::ROW);
         } else if constexpr (V == 4) {
-            const char *at = base + off[j / 4] + 2 * (j % 4) * Im::ROW;
+            const char *at = base + off[j / 4] + (32 * kk + 2 * (j % 4)) * Im::ROW;
             const u32x2 x = *reinterpret_cast<const u32x2 *>(at), y = *reinterpret_cast<const u32x2 *>(at + Im::ROW);
             return u32x4{x[0], x[1], y[0], y[1]};
         } else {
-            const char *at = base + off[j / 2] + 4 * (j % 2) * Im::ROW;
+            const char *at = base + off[j / 2] + (32 * kk + 4 * (j % 2)) * Im::ROW;
             return u32x4{*reinterpret_cast<const uint32_t *>(at), *reinterpret_cast<const uint32_t *>(at + Im::ROW),
                          *reinterpret_cast<const uint32_t *>(at + 2 * Im::ROW), *reinterpret_cast<const uint32_t *>(at + 3 * Im::ROW)};
         }
@@ -279,8 +284,14 @@ template <int X, Lay LAY, int NBLK> struct Fragments {
 
 // Where entry `id` of the list of tiles, batch entries and depth ranges lies.
 struct TileAt {
-    int m0, n0, z, split, first_step, steps;  // steps: even, the last may be empty
-    int64_t depth;                            // bytes from first_step on
+    int m0, n0, z, split, first_step;
+    int steps;        // of the tile
+    int whole, rest;  // steps of 128 bytes from first_step to the end of the depth, and the bytes behind them
+    // Bytes of the depth in step s.
+    __device__ __forceinline__ int bytes(int s) const {
+        const int behind = s == whole ? rest : 0;
+        return s < whole ? 128 : behind;
+    }
 };
 template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p, int id) {
     TileAt t;
@@ -296,9 +307,10 @@ template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p
     t.m0 = (first_m + in_group % gm) * Cfg::BM;
     t.n0 = in_group / gm * Cfg::CHANNELS;
     t.first_step = t.split * p.steps_per_split;
-    t.depth = p.k_bytes - (int64_t)t.first_step * 64;
-    const int64_t all = (t.depth + 127) >> 7 << 1;
-    t.steps = all < p.steps_per_split ? (int)all : p.steps_per_split;
+    t.whole = (int)(p.k_bytes >> 7) - t.first_step;
+    t.rest = (int)(p.k_bytes & 127);
+    const int all = t.whole + (t.rest > 0);
+    t.steps = all < p.steps_per_split ? all : p.steps_per_split;
     return t;
 }
 
@@ -324,8 +336,8 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     const int lda = (int)p.lda, ldb[2] = {(int)p.ldb[0], (int)p.ldb[1]};
     const int a_off = ImA::row_of(0, lane) * lda + a_slot;
     const int b_off[2] = {ImB::row_of(0, lane) * ldb[0] + b_slot, ImB::row_of(0, lane) * ldb[1] + b_slot};
-    const int64_t a_step = Cfg::LAYA == ALONG_K ? 64 : 32 * p.lda;
-    const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 64 : 32 * p.ldb[0], Cfg::LAYB == ALONG_K ? 64 : 32 * p.ldb[1]};
+    const int64_t a_step = Cfg::LAYA == ALONG_K ? 128 : 64 * p.lda;
+    const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[0], Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[1]};
     const char *b_ptr[2] = {static_cast<const char *>(p.B[0]), static_cast<const char *>(p.B[1])};
     const int64_t b_len[2] = {p.b_bytes[0], p.b_bytes[1]};
     constexpr int kOutside = (int)0x80000000u;
@@ -368,11 +380,10 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     // once the last tile has been fed, go out of range, where loads give zeros.  (ACROSS_K: rows behind it lie behind the
     // operand's last byte.)
     auto issue_one = [&](char *dst, int i) {
-        const int64_t left = feed_id < end ? feed.depth - (int64_t)feed_step * 64 : 0;
-        const int depth = left < 64 ? (int)left : 64;
+        const int bytes = feed.bytes(feed_step);  // (none once everything has been fed)
         if (i < LA) {
             const int q = wave + i * Cfg::WAVES;
-            const bool out = Cfg::LAYA == ALONG_K ? a_slot >= depth : feed_id >= end;
+            const bool out = (Cfg::LAYA == ALONG_K ? a_slot : 0) >= bytes;
             const int off = a_off + q * ImA::ROWS_PER_LOAD * lda;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(feed_a, left_a), (lds_void_t *)(dst + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
         } else {
@@ -380,11 +391,11 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
             const int row = q * ImB::ROWS_PER_LOAD;
             const int h = Cfg::GATED ? (row % Cfg::WN) / (Cfg::WN / 2) : 0;
             const int ch = Cfg::GATED ? row / Cfg::WN * (Cfg::WN / 2) + row % (Cfg::WN / 2) : row;
-            const bool out = Cfg::LAYB == ALONG_K ? b_slot >= depth : feed_id >= end;
+            const bool out = (Cfg::LAYB == ALONG_K ? b_slot : 0) >= bytes;
             const bool second = Cfg::GATED ? h : Cfg::PARTS ? part : 0;
             const int off = (second ? b_off[1] : b_off[0]) + ch * (second ? ldb[1] : ldb[0]);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(h ? feed_b[1] : feed_b[0], h ? left_b[1] : left_b[0]),
-                                                     (lds_void_t *)(dst + BM * 64 + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
+                                                     (lds_void_t *)(dst + BM * 128 + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
         }
     };
     auto feed_on = [&] {
@@ -395,6 +406,8 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
             if (feed_id < end) {
                 feed = tile_at<Cfg>(fresh(args), feed_id);
                 aim();
+            } else {
+                feed.whole = -1;
             }
             return;
         }
@@ -412,27 +425,27 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     };
     // A slot that the depth ends in (its last bytes are real memory: the next row) is cut off in LDS once it is there - for
     // both operands, as zero times NaN is no zero.
-    auto cut = [&](char *dst, int q, int slot, int depth) {
-        if (slot != (depth & ~15)) return;
+    auto cut = [&](char *dst, int q, int slot, int bytes) {
+        if (slot != (bytes & ~15)) return;
         u32x4 *at = reinterpret_cast<u32x4 *>(dst + q * 1024 + lane * 16);
         u32x4 v = *at;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int keep = (depth & 15) - 4 * e;  // bytes of this dword
+            const int keep = (bytes & 15) - 4 * e;  // bytes of this dword
             v[e] = keep >= 4 ? v[e] : keep <= 0 ? 0u : v[e] & ((1u << (8 * keep)) - 1);
         }
         *at = v;
     };
-    // What this wave loaded of a step is in LDS: make it fit to be read, then wait for the other waves.  depth: from that
-    // step on.
-    auto publish = [&](char *dst, int64_t depth) {
-        if (depth < 64 && depth > 0 && (depth & 15)) {
+    // What this wave loaded of a step (that holds so many bytes of the depth) is in LDS: make it fit to be read, then wait
+    // for the other waves.
+    auto publish = [&](char *dst, int bytes) {
+        if (bytes & 15) {
             if (Cfg::LAYA == ALONG_K)
 #pragma unroll
-                for (int i = 0; i < LA; ++i) cut(dst, wave + i * Cfg::WAVES, a_slot, (int)depth);
+                for (int i = 0; i < LA; ++i) cut(dst, wave + i * Cfg::WAVES, a_slot, bytes);
             if (Cfg::LAYB == ALONG_K)
 #pragma unroll
-                for (int i = 0; i < LB; ++i) cut(dst + BM * 64, wave + i * Cfg::WAVES, b_slot, (int)depth);
+                for (int i = 0; i < LB; ++i) cut(dst + BM * 128, wave + i * Cfg::WAVES, b_slot, bytes);
         }
         CBA_FFN_WAIT_LDS();  // also: this wave's fragment reads of the stage that is loaded into next have completed
         asm volatile("" ::: "memory");
@@ -444,10 +457,10 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     FragB rb;
     ra.init(lane, wm * Cfg::WM);
     rb.init(lane, wn * Cfg::WN);
-    u32x4 fa[2][TM], fb[2][TN];  // operands of this step and the next
-    auto read_one = [&](const char *stage, int set, int i) {
-        if (i < TN) fb[set][i] = rb.read(stage + BM * 64, i);
-        else fa[set][i - TN] = ra.read(stage, i - TN);
+    u32x4 fa[2][TM], fb[2][TN];  // operands of a step's two MFMAs
+    auto read_one = [&](const char *stage, int kk, int i) {
+        if (i < TN) fb[kk][i] = rb.read(stage + BM * 128, i, kk);
+        else fa[kk][i - TN] = ra.read(stage, i - TN, kk);
     };
     Acc acc[TM][TN];
 
@@ -461,32 +474,39 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     }
     TileAt t = tile_at<Cfg>(fresh(args), id);
     CBA_FFN_WAIT_VM((S - 1) * (LA + LB));
-    publish(lds, t.depth);
+    publish(lds, t.bytes(0));
 #pragma unroll
     for (int i = 0; i < TM + TN; ++i) read_one(lds, 0, i);
 
-    // One step: publish the next one, then multiply this one's operands while the next one's are read and the loads of the
-    // step S later start into the stage that has become free.
-    auto step = [&](int set, int64_t next_depth) {
-        char *next = after(stage);
-        CBA_FFN_WAIT_VM((S - 2) * (LA + LB));
-        publish(next, next_depth);
-        constexpr int OTHER = TM + TN > LA + LB ? TM + TN : LA + LB;
+    // MFMAs kk of a step, with `n` other instructions spread between their rows: behind the first, whose operands are there,
+    // and none behind the last.
+    auto multiply = [&](int kk, int n, auto &&other) {
+        constexpr int ROWS = TM > 1 ? TM - 1 : 1;
 #pragma unroll
-        for (int j = 0; j < TN; j += FragB::V) rb.ready(&fb[set][j]);
+        for (int j = 0; j < TN; j += FragB::V) rb.ready(&fb[kk][j]);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int o = OTHER * i / TM; o < OTHER * (i + 1) / TM; ++o) {
-                if (o < LA + LB) issue_one(stage, o);
-                if (o < TM + TN) read_one(next, set ^ 1, o);
-            }
-            if (i % FragA::V == 0) ra.ready(&fa[set][i]);
+            if (i % FragA::V == 0) ra.ready(&fa[kk][i]);
             // the weights are the instruction's first operand: a lane then holds one token's neighbouring channels
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[set][j], fa[set][i], acc[i][j]);
+            for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[kk][j], fa[kk][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int o = n * i / ROWS; o < n * (i + 1) / ROWS && o < n; ++o) other(o);
         }
+    };
+    // One step: multiply its first half while the second's operands are read; publish the next step; multiply the second
+    // half while the next step's first operands are read and the loads of the step S later start into the stage that has
+    // become free.
+    auto step = [&](int next_bytes) {
+        char *next = after(stage);
+        multiply(0, TM + TN, [&](int o) { read_one(stage, 1, o); });
+        CBA_FFN_WAIT_VM((S - 2) * (LA + LB));
+        publish(next, next_bytes);
+        multiply(1, TM + TN > LA + LB ? TM + TN : LA + LB, [&](int o) {
+            if (o < LA + LB) issue_one(stage, o);
+            if (o < TM + TN) read_one(next, 0, o);
+        });
         feed_on();
         stage = next;
     };
@@ -498,13 +518,8 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
         const int next_id = id + stride;
-        const int64_t next_tile_depth = next_id < end ? tile_at<Cfg>(fresh(args), next_id).depth : 0;
-        int64_t depth = t.depth;
-        for (int s = 0; s < t.steps; s += 2) {
-            step(0, depth - 64);
-            depth -= 128;
-            step(1, s + 2 < t.steps ? depth : next_tile_depth);
-        }
+        const int next_tile_bytes = next_id < end ? tile_at<Cfg>(fresh(args), next_id).bytes(0) : 0;
+        for (int s = 1; s <= t.steps; ++s) step(s < t.steps ? t.bytes(s) : next_tile_bytes);
 
         Args &out = fresh(args);
         // results: four neighbouring columns of a row at a time
