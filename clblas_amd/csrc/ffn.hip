@@ -210,7 +210,7 @@ template <typename Cfg> hipError_t launch_tiles(const Product &p, int K, hipStre
 // The tiled forms: edges, and the index by which a form is known (the forms that run from registers come first).
 enum { ROWS_FORMS = 6 };
 struct TileShape { int bm, bn; };
-const TileShape kTiles[] = {{256, 256}, {256, 128}, {128, 128}, {128, 128}, {64, 128}, {64, 128}, {64, 64}, {128, 256}};
+const TileShape kTiles[] = {{256, 256}, {256, 128}, {128, 128}, {128, 128}, {64, 128}, {64, 128}, {64, 64}, {128, 64}};
 
 template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
     switch (tile) {
@@ -221,7 +221,7 @@ template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(i
     case 4: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED, LA, LB>());
     case 5: return f(TileCfg<ET, 64, 128, 32, 64, 6, GATED, LA, LB>());
     case 6: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED, LA, LB>());
-    default: return f(TileCfg<ET, 128, 256, 64, 64, 3, GATED, LA, LB>());
+    default: return f(TileCfg<ET, 128, 64, 64, 32, 3, GATED, LA, LB>());
     }
 }
 
@@ -249,7 +249,7 @@ TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
         if (splits > 64) splits = 64;
     }
     if (knobs().ffn_splits) splits = knobs().ffn_splits < steps ? knobs().ffn_splits : steps;
-    if (splits < 1) splits = 1;
+    if (splits < 1 || t.bm * t.bn >= 65536) splits = 1;  // (the largest tiles do not split: TileCfg::SPLITS)
     c.steps_per_split = (int)ceil_div(steps, splits);
     c.splits = (int)ceil_div(steps, c.steps_per_split);
     if (c.splits > 1) {

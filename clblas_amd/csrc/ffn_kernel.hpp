@@ -189,6 +189,7 @@ template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay 
     static constexpr int ET = ET_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
     static constexpr bool GATED = GATED_;
     static constexpr Lay LAYA = LAYA_, LAYB = LAYB_;
+    static constexpr bool SPLITS = BM * BN < 65536;    // the depth may be cut into ranges
     static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
     static constexpr int CHANNELS = GATED ? BN / 2 : BN;  // columns of the result per tile
     // B in two parts, one after the other along the depth (the gradient of the input: both weights)
@@ -296,8 +297,11 @@ struct TileAt {
 template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p, int id) {
     TileAt t;
     const int tiles = p.tiles_m * p.tiles_n;
-    t.split = id / (tiles * p.batch);
-    id -= t.split * tiles * p.batch;
+    t.split = 0;
+    if (Cfg::SPLITS) {
+        t.split = id / (tiles * p.batch);
+        id -= t.split * tiles * p.batch;
+    }
     t.z = id / tiles;
     id -= t.z * tiles;
     // groups of group_m tile rows, column by column: tiles that run together share both operands' rows in an L2
@@ -306,13 +310,122 @@ template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p
     const int in_group = id - grp * per_group;
     t.m0 = (first_m + in_group % gm) * Cfg::BM;
     t.n0 = in_group / gm * Cfg::CHANNELS;
-    t.first_step = t.split * p.steps_per_split;
+    t.first_step = Cfg::SPLITS ? t.split * p.steps_per_split : 0;
     t.whole = (int)(p.k_bytes >> 7) - t.first_step;
     t.rest = (int)(p.k_bytes & 127);
     const int all = t.whole + (t.rest > 0);
-    t.steps = all < p.steps_per_split ? all : p.steps_per_split;
+    t.steps = Cfg::SPLITS && all > p.steps_per_split ? p.steps_per_split : all;
     return t;
 }
+
+// From a wave's accumulators to memory.  A lane has four neighbouring columns of a row per quad; two quads make 16 bytes of a
+// 16-bit result.  ALONG_K: quad j holds columns 16 j + 4 g on; lanes 16 apart exchange halves (v_permlane16_swap), after which
+// an even lane group g has columns 4 g .. 4 g + 7 of block j and its odd neighbour those of block j + 1, and a store writes
+// 64 bytes of each of 16 rows.  (8 bytes per lane: 32 bytes a row, 16 x more often half a cache line; gated 8192 x
+// 12288 x 4096 with G and U stored @STORE@.)  ACROSS_K: element e of a quad comes from the e-th block of a group, and two quads
+// are neighbours anyway.
+template <typename Cfg> struct Results {
+    typedef Fragments<Cfg::BM, Cfg::LAYA, Cfg::TM> FragA;
+    static constexpr int V = Fragments<Cfg::BN, Cfg::LAYB, Cfg::TN>::V;
+    static constexpr int QUADS = Cfg::GATED ? Cfg::TN / 2 : Cfg::TN, COLUMNS = 16 * QUADS;  // of a wave
+    typedef typename Mfma<Cfg::ET>::Acc Acc;
+    static __device__ __forceinline__ int column(int j, int g) {
+        return V == 1 ? 16 * j + 4 * g : V == 4 ? j / 4 * 64 + 16 * g + 4 * (j % 4) : j / 2 * 32 + 8 * g + 4 * (j % 2);
+    }
+    static __device__ __forceinline__ Acc quad(const Acc (&acc)[Cfg::TN], int j) {
+        Acc x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = V == 1 ? acc[j][e] : V == 4 ? acc[j / 4 * 4 + e][j % 4] : acc[j / 2 * 2 + (e & 1)][2 * (j % 2) + (e >> 1)];
+        return x;
+    }
+    // Row m's quads to `base` (rows of ld elements, N columns), from column n on.
+    template <int OT> static __device__ __forceinline__ void row(void *base, int64_t ld, int N, int m, int n, int g, const float (&x)[QUADS][4]) {
+        typedef typename Store<OT>::type T;
+        T *to = static_cast<T *>(base) + (int64_t)m * ld;
+        if constexpr (OT != OT_F32 && QUADS % 2 == 0) {
+#pragma unroll
+            for (int j = 0; j < QUADS; j += 2) {
+                union {
+                    T v[8];
+                    uint32_t d[4];
+                } u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u.v[e] = Store<OT>::of(x[j + e / 4][e % 4]);
+                int at = n + column(j, g);
+                if (V == 1) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const auto s = __builtin_amdgcn_permlane16_swap(u.d[h], u.d[2 + h], false, false);
+                        u.d[h] = s[0];
+                        u.d[2 + h] = s[1];
+                    }
+                    at = n + 16 * (j + (g & 1)) + 4 * (g & 2);
+                }
+                if (at + 8 <= N) {
+                    __builtin_memcpy(to + at, u.v, 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 7; ++e)
+                        if (at + e < N) to[at + e] = u.v[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < QUADS; ++j)
+                if (n + column(j, g) < N) store4_as<OT>(to, n + column(j, g), x[j], N - n - column(j, g));
+        }
+    }
+    template <int OT>
+    static __device__ __forceinline__ void store(Args &p, const TileAt &t, const Acc (&acc)[Cfg::TM][Cfg::TN], int wm, int wn, int r, int g) {
+        const int N = p.N, n = t.n0 + wn * COLUMNS;
+        constexpr int FACTORS = Cfg::GATED ? 2 : 1;
+        float scale[FACTORS][QUADS][4];  // of the channels
+        if (Cfg::ET == ET_I8) {
+#pragma unroll
+            for (int h = 0; h < FACTORS; ++h)
+#pragma unroll
+                for (int j = 0; j < QUADS; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = n + column(j, g) + e;
+                        scale[h][j][e] = p.scale_b[h][c < N ? c : N - 1];
+                    }
+        }
+#pragma unroll
+        for (int i = 0; i < Cfg::TM; ++i) {
+            const int m = t.m0 + wm * Cfg::WM + FragA::row(i, r);
+            const bool there = m < p.M;  // (lanes stay together for the exchange)
+            float x[QUADS][4], u[QUADS][4];
+            float sa = 1.f;
+            if (Cfg::ET == ET_I8) sa = p.scale_a[there ? m : p.M - 1];
+#pragma unroll
+            for (int j = 0; j < QUADS; ++j) {
+                const Acc q = quad(acc[i], j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[j][e] = (float)q[e];
+                    if (Cfg::ET == ET_I8) x[j][e] = x[j][e] * sa * scale[0][j][e];
+                    if (Cfg::GATED) {
+                        u[j][e] = (float)acc[i][j + Cfg::TN / 2][e];
+                        if (Cfg::ET == ET_I8) u[j][e] = u[j][e] * sa * scale[FACTORS - 1][j][e];
+                    }
+                }
+            }
+            const int last = there ? N : 0;  // (a row that is not there has no columns)
+            if (Cfg::GATED) {
+                if (p.save[0]) {
+                    row<OT>(p.save[0], p.ld_save[0], last, m, n, g, x);
+                    row<OT>(p.save[1], p.ld_save[1], last, m, n, g, u);
+                }
+#pragma unroll
+                for (int j = 0; j < QUADS; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[j][e] = gate_value(p.gate, x[j][e]) * u[j][e];
+            }
+            row<OT>(p.C[t.z], p.ldc[t.z], last, m, n, g, x);
+        }
+    }
+};
 
 // Tiles id, id + stride, ... below `end`.
 template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *args, int id, int stride, int end, char *lds) {
@@ -323,6 +436,7 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     typedef Image<BN, Cfg::LAYB> ImB;
     typedef Fragments<BM, Cfg::LAYA, TM> FragA;
     typedef Fragments<BN, Cfg::LAYB, TN> FragB;
+    typedef Results<Cfg> Res;
     if (id >= end) return;
     Args &p = *args;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -338,89 +452,87 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     const int b_off[2] = {ImB::row_of(0, lane) * ldb[0] + b_slot, ImB::row_of(0, lane) * ldb[1] + b_slot};
     const int64_t a_step = Cfg::LAYA == ALONG_K ? 128 : 64 * p.lda;
     const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[0], Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[1]};
-    const char *b_ptr[2] = {static_cast<const char *>(p.B[0]), static_cast<const char *>(p.B[1])};
+    const char *b_from[2] = {static_cast<const char *>(p.B[0]), static_cast<const char *>(p.B[1])};
     const int64_t b_len[2] = {p.b_bytes[0], p.b_bytes[1]};
     constexpr int kOutside = (int)0x80000000u;
 
-    // The feeding side runs S steps ahead of the multiplying one.  feed_*: operands from the next step on.
-    TileAt feed = tile_at<Cfg>(fresh(args), id);
-    int feed_id = id, feed_step = 0, part = 0;
-    const char *feed_a, *feed_b[2];
-    int64_t left_a, left_b[2];
-    auto aim_b = [&](int h, int step) {  // at a step within B[h]
-        Args &p = fresh(args);
-        const int64_t skip = (Cfg::LAYB == ALONG_K ? feed.n0 * p.ldb[h] : (int64_t)feed.n0 * 2) + step * b_step[h];
-        const int to = Cfg::GATED ? h : 0;
-        feed_b[to] = static_cast<const char *>(p.B[h]) + skip;
-        left_b[to] = p.b_bytes[h] - skip;
-    };
-    // (PARTS: aimed anew for every step, without a branch)
+    // The feeding side runs S steps ahead of the multiplying one: the next step to load, and its place in memory.
+    // (While a step is within a tile the places only move on; no branch chooses between them.)
     const int part_steps = Cfg::PARTS ? p.part_steps : 0;
-    auto aim_parts = [&] {
+    TileAt feed = tile_at<Cfg>(fresh(args), id);
+    int feed_id = id, feed_step = 0;
+    const char *a_ptr, *b_ptr[2];
+    int64_t a_left, b_left[2];
+    int part = 0;
+    auto aim_a = [&] {
+        Args &p = fresh(args);
+        const int64_t skip = (Cfg::LAYA == ALONG_K ? feed.m0 * p.lda : (int64_t)feed.m0 * 2) + feed.first_step * a_step;
+        a_ptr = static_cast<const char *>(p.A[feed.z]) + skip;
+        a_left = p.a_bytes - skip;
+    };
+    auto aim_parts = [&] {  // PARTS: anew for every step
         const int step = feed.first_step + feed_step;
         part = step >= part_steps;
         const int64_t skip = (int64_t)feed.n0 * 2 + (int64_t)(part ? step - part_steps : step) * (part ? b_step[1] : b_step[0]);
-        feed_b[0] = (part ? b_ptr[1] : b_ptr[0]) + skip;
-        left_b[0] = (part ? b_len[1] : b_len[0]) - skip;
+        b_ptr[0] = (part ? b_from[1] : b_from[0]) + skip;
+        b_left[0] = (part ? b_len[1] : b_len[0]) - skip;
     };
-    auto aim = [&] {
-        Args &p = fresh(args);
-        const int64_t skip = (Cfg::LAYA == ALONG_K ? feed.m0 * p.lda : (int64_t)feed.m0 * 2) + feed.first_step * a_step;
-        feed_a = static_cast<const char *>(p.A[feed.z]) + skip;
-        left_a = p.a_bytes - skip;
+    auto aim_b = [&] {
         if constexpr (Cfg::PARTS) {
             aim_parts();
         } else {
-            aim_b(0, feed.first_step);
-            if (Cfg::GATED) aim_b(1, feed.first_step);
+            Args &p = fresh(args);
+#pragma unroll
+            for (int h = 0; h < (Cfg::GATED ? 2 : 1); ++h) {
+                const int64_t skip = (Cfg::LAYB == ALONG_K ? feed.n0 * p.ldb[h] : (int64_t)feed.n0 * 2) + feed.first_step * b_step[h];
+                b_ptr[h] = static_cast<const char *>(p.B[h]) + skip;
+                b_left[h] = p.b_bytes[h] - skip;
+            }
         }
     };
-    aim();
-    // Starts one of the LA + LB loads of the feeding side's step.  ALONG_K: slots behind the depth's end, and everything
-    // once the last tile has been fed, go out of range, where loads give zeros.  (ACROSS_K: rows behind it lie behind the
-    // operand's last byte.)
-    auto issue_one = [&](char *dst, int i) {
-        const int bytes = feed.bytes(feed_step);  // (none once everything has been fed)
-        if (i < LA) {
-            const int q = wave + i * Cfg::WAVES;
-            const bool out = (Cfg::LAYA == ALONG_K ? a_slot : 0) >= bytes;
-            const int off = a_off + q * ImA::ROWS_PER_LOAD * lda;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(feed_a, left_a), (lds_void_t *)(dst + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
-        } else {
-            const int q = wave + (i - LA) * Cfg::WAVES;
-            const int row = q * ImB::ROWS_PER_LOAD;
-            const int h = Cfg::GATED ? (row % Cfg::WN) / (Cfg::WN / 2) : 0;
-            const int ch = Cfg::GATED ? row / Cfg::WN * (Cfg::WN / 2) + row % (Cfg::WN / 2) : row;
-            const bool out = (Cfg::LAYB == ALONG_K ? b_slot : 0) >= bytes;
-            const bool second = Cfg::GATED ? h : Cfg::PARTS ? part : 0;
-            const int off = (second ? b_off[1] : b_off[0]) + ch * (second ? ldb[1] : ldb[0]);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(h ? feed_b[1] : feed_b[0], h ? left_b[1] : left_b[0]),
-                                                     (lds_void_t *)(dst + BM * 128 + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
-        }
+    aim_a();
+    aim_b();
+    // One of the loads of an operand's next step.  ALONG_K: slots behind the depth's end, and everything once the last tile has
+    // been fed, go out of range, where loads give zeros.  (ACROSS_K: rows behind it lie behind the operand's last byte.)
+    auto load_a = [&](char *dst, int i) {
+        const int q = wave + i * Cfg::WAVES;
+        const bool out = (Cfg::LAYA == ALONG_K ? a_slot : 0) >= feed.bytes(feed_step);
+        const int off = a_off + q * ImA::ROWS_PER_LOAD * lda;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(a_ptr, a_left), (lds_void_t *)(dst + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
+    };
+    auto load_b = [&](char *dst, int i) {
+        const int q = wave + i * Cfg::WAVES, row = q * ImB::ROWS_PER_LOAD;
+        const int h = Cfg::GATED ? (row % Cfg::WN) / (Cfg::WN / 2) : 0;
+        const int ch = Cfg::GATED ? row / Cfg::WN * (Cfg::WN / 2) + row % (Cfg::WN / 2) : row;
+        const bool out = (Cfg::LAYB == ALONG_K ? b_slot : 0) >= feed.bytes(feed_step);
+        const bool second = Cfg::GATED ? h : Cfg::PARTS ? part : 0;
+        const int off = (second ? b_off[1] : b_off[0]) + ch * (second ? ldb[1] : ldb[0]);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(h ? b_ptr[1] : b_ptr[0], h ? b_left[1] : b_left[0]), (lds_void_t *)(dst + q * 1024), 16,
+                                                 out ? kOutside : off, 0, 0, 0);
     };
     auto feed_on = [&] {
-        ++feed_step;
-        if (feed_step == feed.steps) {
-            feed_id += stride;
-            feed_step = 0;
-            if (feed_id < end) {
-                feed = tile_at<Cfg>(fresh(args), feed_id);
-                aim();
+        if (++feed_step < feed.steps) {
+            a_ptr += a_step;
+            a_left -= a_step;
+            if constexpr (Cfg::PARTS) {
+                aim_parts();
             } else {
-                feed.whole = -1;
+#pragma unroll
+                for (int h = 0; h < (Cfg::GATED ? 2 : 1); ++h) {
+                    b_ptr[h] += b_step[h];
+                    b_left[h] -= b_step[h];
+                }
             }
             return;
         }
-        feed_a += a_step;
-        left_a -= a_step;
-        if constexpr (Cfg::PARTS) {
-            aim_parts();
+        feed_step = 0;
+        feed_id += stride;
+        if (feed_id < end) {
+            feed = tile_at<Cfg>(fresh(args), feed_id);
+            aim_a();
+            aim_b();
         } else {
-#pragma unroll
-            for (int h = 0; h < (Cfg::GATED ? 2 : 1); ++h) {
-                feed_b[h] += b_step[h];
-                left_b[h] -= b_step[h];
-            }
+            feed.whole = -1;
         }
     };
     // A slot that the depth ends in (its last bytes are real memory: the next row) is cut off in LDS once it is there - for
@@ -438,14 +550,14 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     };
     // What this wave loaded of a step (that holds so many bytes of the depth) is in LDS: make it fit to be read, then wait
     // for the other waves.
-    auto publish = [&](char *dst, int bytes) {
+    auto publish = [&](char *at, int bytes) {
         if (bytes & 15) {
             if (Cfg::LAYA == ALONG_K)
 #pragma unroll
-                for (int i = 0; i < LA; ++i) cut(dst, wave + i * Cfg::WAVES, a_slot, bytes);
+                for (int i = 0; i < LA; ++i) cut(at, wave + i * Cfg::WAVES, a_slot, bytes);
             if (Cfg::LAYB == ALONG_K)
 #pragma unroll
-                for (int i = 0; i < LB; ++i) cut(dst + BM * 128, wave + i * Cfg::WAVES, b_slot, bytes);
+                for (int i = 0; i < LB; ++i) cut(at + BM * 128, wave + i * Cfg::WAVES, b_slot, bytes);
         }
         CBA_FFN_WAIT_LDS();  // also: this wave's fragment reads of the stage that is loaded into next have completed
         asm volatile("" ::: "memory");
@@ -458,18 +570,20 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     ra.init(lane, wm * Cfg::WM);
     rb.init(lane, wn * Cfg::WN);
     u32x4 fa[2][TM], fb[2][TN];  // operands of a step's two MFMAs
-    auto read_one = [&](const char *stage, int kk, int i) {
-        if (i < TN) fb[kk][i] = rb.read(stage + BM * 128, i, kk);
-        else fa[kk][i - TN] = ra.read(stage, i - TN, kk);
+    auto read_one = [&](const char *at, int kk, int i) {
+        if (i < TN) fb[kk][i] = rb.read(at + BM * 128, i, kk);
+        else fa[kk][i - TN] = ra.read(at, i - TN, kk);
     };
     Acc acc[TM][TN];
 
     char *stage = lds;
-    auto after = [&](char *st) { return st + Cfg::STAGE == lds + Cfg::LDS ? lds : st + Cfg::STAGE; };
+    auto after = [&](char *at) { return at + Cfg::STAGE == lds + Cfg::LDS ? lds : at + Cfg::STAGE; };
 #pragma nounroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-        for (int i = 0; i < LA + LB; ++i) issue_one(lds + s * Cfg::STAGE, i);
+        for (int i = 0; i < LA; ++i) load_a(lds + s * Cfg::STAGE, i);
+#pragma unroll
+        for (int i = 0; i < LB; ++i) load_b(lds + s * Cfg::STAGE + BM * 128, i);
         feed_on();
     }
     TileAt t = tile_at<Cfg>(fresh(args), id);
@@ -478,9 +592,9 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
 #pragma unroll
     for (int i = 0; i < TM + TN; ++i) read_one(lds, 0, i);
 
-    // MFMAs kk of a step, with `n` other instructions spread between their rows: behind the first, whose operands are there,
-    // and none behind the last.
-    auto multiply = [&](int kk, int n, auto &&other) {
+    // MFMAs kk of a step.  Loads and reads are spread between their rows: behind the first, whose operands are there, and
+    // none behind the last.
+    auto multiply = [&](int kk, int loads, int reads, auto &&load, auto &&read) {
         constexpr int ROWS = TM > 1 ? TM - 1 : 1;
 #pragma unroll
         for (int j = 0; j < TN; j += FragB::V) rb.ready(&fb[kk][j]);
@@ -491,22 +605,22 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[kk][j], fa[kk][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
+            if (i >= ROWS) continue;
 #pragma unroll
-            for (int o = n * i / ROWS; o < n * (i + 1) / ROWS && o < n; ++o) other(o);
+            for (int o = loads * i / ROWS; o < loads * (i + 1) / ROWS; ++o) load(o);
+#pragma unroll
+            for (int o = reads * i / ROWS; o < reads * (i + 1) / ROWS; ++o) read(o);
         }
     };
     // One step: multiply its first half while the second's operands are read; publish the next step; multiply the second
-    // half while the next step's first operands are read and the loads of the step S later start into the stage that has
-    // become free.
+    // half while the next step's first operands are read and the loads of the step S later start into the stage that is free.
     auto step = [&](int next_bytes) {
-        char *next = after(stage);
-        multiply(0, TM + TN, [&](int o) { read_one(stage, 1, o); });
+        char *const next = after(stage), *const free = stage;
+        multiply(0, 0, TM + TN, [&](int) {}, [&](int o) { read_one(free, 1, o); });
         CBA_FFN_WAIT_VM((S - 2) * (LA + LB));
         publish(next, next_bytes);
-        multiply(1, TM + TN > LA + LB ? TM + TN : LA + LB, [&](int o) {
-            if (o < LA + LB) issue_one(stage, o);
-            if (o < TM + TN) read_one(next, 0, o);
-        });
+        multiply(1, LA + LB, TM + TN, [&](int o) { o < LA ? load_a(free, o) : load_b(free + BM * 128, o - LA); },
+                 [&](int o) { read_one(next, 0, o); });
         feed_on();
         stage = next;
     };
@@ -522,39 +636,35 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
         for (int s = 1; s <= t.steps; ++s) step(s < t.steps ? t.bytes(s) : next_tile_bytes);
 
         Args &out = fresh(args);
-        // results: four neighbouring columns of a row at a time
-        constexpr int HALF = Cfg::GATED ? TN / 2 : TN, J2 = Cfg::GATED ? HALF : 0;
+        if (out.splits > 1) {
+            // partial sums, four neighbouring columns of a row at a time
+            typedef typename ElemOf<Cfg::ET>::Acc Sum;
+            Sum *const ws = reinterpret_cast<Sum *>(out.ws) + (int64_t)t.split * out.ws_split + (int64_t)t.z * out.ws_plane;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int m = t.m0 + wm * Cfg::WM + FragA::row(i, r);
-            if (m >= out.M) continue;
+            for (int i = 0; i < TM; ++i) {
+                const int m = t.m0 + wm * Cfg::WM + FragA::row(i, r);
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) {
-                // ALONG_K: the four elements of accumulator j; else element e comes from the e-th block of a group
-                constexpr int V = FragB::V;
-                const int n = t.n0 + wn * (HALF * 16) + (V == 1 ? 16 * j + 4 * g : V == 4 ? j / 4 * 64 + 16 * g + 4 * (j % 4) : j / 2 * 32 + 8 * g + 4 * (j % 2));
-                if (n >= out.N) continue;
-                Acc x, u;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = V == 1 ? acc[i][j][e] : V == 4 ? acc[i][j / 4 * 4 + e][j % 4] : acc[i][j / 2 * 2 + (e & 1)][2 * (j % 2) + (e >> 1)];
-                    u[e] = acc[i][j + J2][e];
-                }
-                if (out.splits > 1) {
-                    typedef typename ElemOf<Cfg::ET>::Acc Sum;
-                    Sum *w = reinterpret_cast<Sum *>(out.ws) + (int64_t)t.split * out.ws_split + (int64_t)t.z * out.ws_plane + (int64_t)m * out.ws_ld + n;
-                    *reinterpret_cast<Acc *>(w) = x;
-                    if (Cfg::GATED) *reinterpret_cast<Acc *>(w + out.ws_plane) = u;
-                } else {
-                    const float fx[4] = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-                    const float fu[4] = {(float)u[0], (float)u[1], (float)u[2], (float)u[3]};
-                    finish4<Cfg::ET, Cfg::GATED>(out, t.z, m, n, fx, fu);
+                for (int j = 0; j < Res::QUADS; ++j) {
+                    const int n = t.n0 + wn * Res::COLUMNS + Res::column(j, g);
+                    if (m >= out.M || n >= out.N) continue;
+                    Sum *w = ws + (int64_t)m * out.ws_ld + n;
+                    *reinterpret_cast<Acc *>(w) = Res::quad(acc[i], j);
+                    if (Cfg::GATED) *reinterpret_cast<Acc *>(w + out.ws_plane) = acc[i][j + TN / 2];
                 }
             }
+        } else if (Cfg::ET == ET_F16 || (Cfg::ET == ET_I8 && out.out_type == OT_F16)) {
+            if (Cfg::ET != ET_BF16) Res::template store<OT_F16>(out, t, acc, wm, wn, r, g);
+        } else if (Cfg::ET == ET_BF16 || out.out_type == OT_BF16) {
+            if (Cfg::ET != ET_F16) Res::template store<OT_BF16>(out, t, acc, wm, wn, r, g);
+        } else {
+            if (Cfg::ET == ET_I8) Res::template store<OT_F32>(out, t, acc, wm, wn, r, g);
         }
         if (next_id >= end) break;
         id = next_id;
         t = tile_at<Cfg>(fresh(args), id);
+        // (read once more: kept over the stores, these registers would be spilled)
+#pragma unroll
+        for (int i = 0; i < TM + TN; ++i) read_one(stage, 0, i);
     }
     CBA_FFN_WAIT_VM(0);  // (nothing may be on its way into LDS when the workgroup ends)
 }
