@@ -195,60 +195,43 @@ hipError_t launched(const char *kernel, char type, int bm, int bn, int threads, 
 
 char type_letter(int et) { return et == ET_I8 ? 'i' : et == ET_F16 ? 'h' : 'b'; }
 
-template <typename Cfg> hipError_t launch_tiles(const Product &p, int K, hipStream_t stream) {
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
-    if (tiles > 0x7fffffff - 65536) return hipErrorNotSupported;
-    // as many workgroups as the card holds at once
-    const int per_cu = 160 * 1024 / Cfg::LDS < 8 / Cfg::WAVES ? 160 * 1024 / Cfg::LDS : 8 / Cfg::WAVES;
-    const unsigned grid = (unsigned)(tiles < 256 * per_cu ? tiles : 256 * per_cu);
-    hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<Cfg>, Cfg::LDS);
-    if (e != hipSuccess) return e;
-    e = launch_kernel(tile_kernel<Cfg>, dim3(grid), dim3(Cfg::THREADS), Cfg::LDS, stream, p);
-    return launched("ffn_tile_kernel", type_letter(Cfg::ET), Cfg::BM, Cfg::CHANNELS, Cfg::THREADS, p.M, p.N, K, grid, 1, p.splits, e);
-}
-
-// The tiled forms: edges, and the index by which a form is known (the forms that run from registers come first).
-enum { ROWS_FORMS = 6 };
-struct TileShape { int bm, bn; };
-const TileShape kTiles[] = {{256, 256}, {256, 128}, {128, 128}, {128, 128}, {64, 128}, {64, 128}, {64, 64}, {128, 64}};
+// The forms of a product: those that run from registers (workgroups of 16 TM x 16 TN results - gated: of either factor - on
+// W waves), then the tiled ones.
+struct RowsShape { int tm, tn; };
+const RowsShape kRows[] = {{1, 1}, {2, 1}, {2, 2}, {4, 2}};
+enum { ROWS_FORMS = 4, TILE_FORMS = 5 };
+// step: us per step of 128 bytes of depth, alone on a CU / per tile where more tiles than CUs keep it busy; per_cu: workgroups
+// that a CU holds.  Measured on products of 128 ... 8192 rows, 1024 ... 12288 channels, 1024 ... 8192 deep (alone: e.g. 64 x 64
+// at 256 x 1024 x 4096 8-bit, 32 steps in 14.9 us; busy: 64 x 128 at 1024 x 4096 x 4096 gated, 4 x 64 steps per CU in 102 us).
+struct TileShape { int bm, bn, per_cu; double step_alone, step_busy; };
+const TileShape kTiles[TILE_FORMS] = {
+    {256, 256, 1, 1.50, 1.62}, {256, 128, 1, 0.87, 0.97}, {128, 128, 2, 0.97, 0.57}, {64, 128, 2, 0.50, 0.375}, {64, 64, 2, 0.36, 0.27}};
 
 template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
     switch (tile) {
     case 0: return f(TileCfg<ET, 256, 256, 128, 64, 2, GATED, LA, LB>());
     case 1: return f(TileCfg<ET, 256, 128, 64, 64, 3, GATED, LA, LB>());
-    case 2: return f(TileCfg<ET, 128, 128, 64, 64, 5, GATED, LA, LB>());
-    case 3: return f(TileCfg<ET, 128, 128, 64, 64, 2, GATED, LA, LB>());
-    case 4: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED, LA, LB>());
-    case 5: return f(TileCfg<ET, 64, 128, 32, 64, 6, GATED, LA, LB>());
-    case 6: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED, LA, LB>());
-    default: return f(TileCfg<ET, 128, 64, 64, 32, 3, GATED, LA, LB>());
+    case 2: return f(TileCfg<ET, 128, 128, 64, 64, 2, GATED, LA, LB>());
+    case 3: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED, LA, LB>());
+    default: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED, LA, LB>());
     }
 }
 
-struct TileChoice {
-    int tile = 0, tiles_m = 0, tiles_n = 0, splits = 1, steps_per_split = 0;
+// How one product is tiled.
+struct Tiling {
+    int tiles_m = 0, tiles_n = 0, batch = 1, splits = 1, steps_per_split = 0;
     int64_t ws_ld = 0, ws_plane = 0, ws_split = 0;
     size_t ws_bytes = 0;
+    int64_t count() const { return (int64_t)tiles_m * tiles_n * batch * splits; }
 };
-
-// The 256 x 256 tile where its tiles fill the 256 CUs, else 128 x 128, with the depth cut into ranges (of at least four
-// steps) until they do.
-TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
-    TileChoice c;
+Tiling tiling(int tile, bool gated, int M, int N, int batch, int64_t k_bytes, int splits) {
+    Tiling c;
+    const TileShape &t = kTiles[tile];
     const int64_t steps = ceil_div(k_bytes, 128);
-    auto tiles = [&](int bm, int bn) { return ceil_div(M, bm) * ceil_div(N, gated ? bn / 2 : bn) * batch; };
-    c.tile = tiles(256, 256) >= 256 ? 0 : 2;
-    if (knobs().ffn_form >= ROWS_FORMS) c.tile = knobs().ffn_form - ROWS_FORMS;
-    const TileShape t = kTiles[c.tile];
     c.tiles_m = (int)ceil_div(M, t.bm);
     c.tiles_n = (int)ceil_div(N, gated ? t.bn / 2 : t.bn);
-    int64_t splits = 1;
-    if (t.bm * t.bn < 65536) {
-        splits = 512 / tiles(t.bm, t.bn);
-        if (splits > steps / 4) splits = steps / 4;
-        if (splits > 64) splits = 64;
-    }
-    if (knobs().ffn_splits) splits = knobs().ffn_splits < steps ? knobs().ffn_splits : steps;
+    c.batch = batch;
+    if (splits > steps) splits = (int)steps;
     if (splits < 1 || t.bm * t.bn >= 65536) splits = 1;  // (the largest tiles do not split: TileCfg::SPLITS)
     c.steps_per_split = (int)ceil_div(steps, splits);
     c.splits = (int)ceil_div(steps, c.steps_per_split);
@@ -261,9 +244,78 @@ TileChoice choose(bool gated, int M, int N, int batch, int64_t k_bytes) {
     return c;
 }
 
-template <int ET, bool GATED, Lay LA, Lay LB> hipError_t run_product(Product p, const TileChoice &c, uint32_t *ws, int K, hipStream_t stream) {
+// Time (us) of a launch over tilings that share it: the steps that the busiest of 256 CUs goes through, about 4.5 us for the
+// launch, the first loads and the results, and for sums in pieces a second launch (3 us) and the partial sums, written and
+// read again, at 0.6 us per MB (256 x 4096 x 4096 gated in two ranges of 64 x 128 tiles: 16.8 MB, 43.5 us; in one, 36.7).
+double tiled_cost(int tile, const Tiling *c, int n) {
+    const TileShape &t = kTiles[tile];
+    double count = 0, steps = 0, longest = 0, partial = 0;
+    for (int i = 0; i < n; ++i) {
+        count += (double)c[i].count();
+        steps += (double)c[i].count() * c[i].steps_per_split;
+        if (c[i].count() && c[i].steps_per_split > longest) longest = c[i].steps_per_split;
+        partial += (double)c[i].ws_bytes;
+    }
+    double time;
+    if (count <= 256) time = longest * t.step_alone;
+    else if (n == 1) time = (double)ceil_div((int64_t)count, 256) * longest * t.step_busy;
+    else time = (steps / 256 > longest ? steps / 256 : longest) * t.step_busy;
+    return 4.5 + time + (partial > 0 ? 3.0 + partial * 0.6e-6 : 0.0);
+}
+
+const int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+
+// A form for a whole product, and its time by the model.
+struct Choice {
+    int form = 0;
+    Tiling tiling;
+    double cost = 1e30;
+};
+
+// From registers: what the busiest CU reads, at 33 bytes per ns (measured for workgroups of 16 x 16 ... 64 x 32 results,
+// gated and 8-bit, 16 ... 256 rows; within 10 %), or the weights from memory at 5.4 TB/s; 2.8 us for the launch.
+double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes) {
+    const int64_t groups = ceil_div(M, 16 * s.tm) * ceil_div(N, 16 * s.tn);
+    const int64_t rows = (M < 16 * s.tm ? M : 16 * s.tm) + 16 * s.tn * (gated ? 2 : 1);
+    const double cu = (double)ceil_div(groups, 256) * rows * k_bytes / 33e3;
+    const double memory = ((double)M + (double)N * (gated ? 2 : 1)) * k_bytes / 5.4e6;
+    return 2.8 + (cu > memory ? cu : memory);
+}
+
+// copied: bytes that a tiled form would have to copy first (0.4 us per MB and a launch), where the registers form reads
+// anything as it is.  tiled: whether the rows are short enough for the tiled forms.
+Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool tiled) {
+    Choice best;
+    const int forced = knobs().ffn_form;
+    for (int i = 0; i < ROWS_FORMS; ++i) {
+        const double cost = rows_cost(kRows[i], gated, M, N, k_bytes);
+        if (forced >= 0 ? forced == i || (!tiled && i == 0) : cost < best.cost) {
+            best.form = i;
+            best.cost = cost;
+        }
+    }
+    if (!tiled) return best;
+    for (int i = 0; i < TILE_FORMS; ++i) {
+        if (forced >= 0 && forced != ROWS_FORMS + i) continue;
+        for (int splits : kSplits) {
+            if (knobs().ffn_splits && splits != 1) break;
+            const Tiling t = tiling(i, gated, M, N, 1, k_bytes, knobs().ffn_splits ? knobs().ffn_splits : splits);
+            if (t.splits != splits && !knobs().ffn_splits) break;
+            const double cost = tiled_cost(i, &t, 1) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
+            if (cost < best.cost || (forced >= 0 && best.form != forced)) {
+                best.form = ROWS_FORMS + i;
+                best.tiling = t;
+                best.cost = cost;
+            }
+        }
+    }
+    return best;
+}
+
+Product tiled_product(Product p, const Tiling &c, uint32_t *ws) {
     p.tiles_m = c.tiles_m;
     p.tiles_n = c.tiles_n;
+    p.batch = c.batch;
     p.group_m = 8;
     p.splits = c.splits;
     p.steps_per_split = c.steps_per_split;
@@ -271,10 +323,32 @@ template <int ET, bool GATED, Lay LA, Lay LB> hipError_t run_product(Product p, 
     p.ws_ld = c.ws_ld;
     p.ws_plane = c.ws_plane;
     p.ws_split = c.ws_split;
-    hipError_t e = with_tile<ET, GATED, LA, LB>(c.tile, [&](auto cfg) { return launch_tiles<decltype(cfg)>(p, K, stream); });
+    return p;
+}
+
+// Workgroups that the card holds at once.
+template <typename Cfg> constexpr int resident() {
+    constexpr int by_lds = 160 * 1024 / Cfg::LDS, by_waves = 8 / Cfg::WAVES;
+    return 256 * (by_lds < by_waves ? by_lds : by_waves);
+}
+
+unsigned join_grid(const Product &p) {
+    const int64_t work = (p.ws_ld >> 2) * p.M * p.batch;
+    return (unsigned)(ceil_div(work, 256) < 2048 ? ceil_div(work, 256) : 2048);
+}
+
+template <int ET, bool GATED> hipError_t run_tiles(const Product &p, int tile, int K, hipStream_t stream) {
+    hipError_t e = with_tile<ET, GATED, ALONG_K, ALONG_K>(tile, [&](auto cfg) {
+        typedef decltype(cfg) Cfg;
+        const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
+        if (tiles > 0x7fffffff - 65536) return hipErrorNotSupported;
+        const unsigned grid = (unsigned)(tiles < resident<Cfg>() ? tiles : resident<Cfg>());
+        hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<Cfg>, Cfg::LDS);
+        if (e == hipSuccess) e = launch_kernel(tile_kernel<Cfg>, dim3(grid), dim3(Cfg::THREADS), Cfg::LDS, stream, p);
+        return launched("ffn_tile_kernel", type_letter(ET), Cfg::BM, Cfg::CHANNELS, Cfg::THREADS, p.M, p.N, K, grid, 1, p.splits, e);
+    });
     if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t work = (c.ws_ld >> 2) * p.M * p.batch;
-    const unsigned grid = (unsigned)(ceil_div(work, 256) < 2048 ? ceil_div(work, 256) : 2048);
+    const unsigned grid = join_grid(p);
     e = launch_kernel(join_kernel<ET, GATED>, dim3(grid), dim3(256), 0, stream, p);
     return launched("ffn_join_kernel", type_letter(ET), 1, 4, 256, p.M, p.N, K, grid, 1, p.splits, e);
 }
@@ -282,6 +356,7 @@ template <int ET, bool GATED, Lay LA, Lay LB> hipError_t run_product(Product p, 
 template <typename Cfg> hipError_t launch_rows(Product p, int K, hipStream_t stream) {
     p.tiles_m = (int)ceil_div(p.M, 16 * Cfg::TM);
     p.tiles_n = (int)ceil_div(p.N, 16 * Cfg::TN);
+    p.batch = p.splits = 1;
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
     if (grid * Cfg::THREADS > 0xffffffffLL) return hipErrorNotSupported;
     if (Cfg::LDS > 65536) {
@@ -297,9 +372,7 @@ template <int ET, bool GATED> hipError_t run_rows(const Product &p, int form, in
     case 0: return launch_rows<RowsCfg<ET, 1, 1, 8, 4, GATED>>(p, K, stream);
     case 1: return launch_rows<RowsCfg<ET, 2, 1, 8, 4, GATED>>(p, K, stream);
     case 2: return launch_rows<RowsCfg<ET, 2, 2, 8, 2, GATED>>(p, K, stream);
-    case 3: return launch_rows<RowsCfg<ET, 4, 1, 8, 2, GATED>>(p, K, stream);
-    case 4: return launch_rows<RowsCfg<ET, 4, 2, 4, 2, GATED>>(p, K, stream);
-    default: return launch_rows<RowsCfg<ET, 4, GATED ? 2 : 4, 4, 2, GATED>>(p, K, stream);
+    default: return launch_rows<RowsCfg<ET, 4, 2, 4, 2, GATED>>(p, K, stream);
     }
 }
 
@@ -316,7 +389,7 @@ struct Copies {
 // Whether the tiled product can load an operand from where it is: dword-aligned rows, near enough to each other for 32-bit
 // offsets across a tile.
 bool fits(const void *ptr, int64_t ld_bytes) {
-    return (reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && (ld_bytes & 3) == 0 && ld_bytes < ((int64_t)1 << 22);
+    return (reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && (ld_bytes & 3) == 0 && ld_bytes <= kMaxRowBytes;
 }
 
 hipError_t pack_rows(const void *from, int64_t ld, int64_t bytes, char *to, int64_t ld_to, int64_t rows, hipStream_t stream) {
@@ -326,66 +399,79 @@ hipError_t pack_rows(const void *from, int64_t ld, int64_t bytes, char *to, int6
     return launched("ffn_pack_rows_kernel", 'p', 1, 16, 256, (int)rows, (int)bytes, 0, grid, 1, 1, e);
 }
 
-// A product whose operands are the caller's: copies the ones that do not fit, then runs it.
+// A product whose operands are the caller's: chooses its form, copies what that form cannot load, and runs it.
 template <int ET, bool GATED>
 hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Product p, hipStream_t stream) {
+    constexpr int OPERANDS = GATED ? 3 : 2;
     const int64_t kb = (int64_t)K * es, kp = round_up(kb, 16);
-    Mat in[3] = {A, B0, B1};
-    const int form = knobs().ffn_form;
-    if (form >= 0 && form < ROWS_FORMS) {
-        p.A[0] = A.ptr;
-        p.lda = A.ld * es;
-        p.B[0] = B0.ptr;
-        p.B[1] = B1.ptr;
-        p.ldb[0] = B0.ld * es;
-        p.ldb[1] = B1.ld * es;
-        p.k_bytes = kb;
-        p.M = M;
-        p.N = N;
-        p.batch = 1;
-        return run_rows<ET, GATED>(p, form, K, stream);
-    }
+    const Mat in[3] = {A, B0, B1};
     const int64_t rows[3] = {M, N, N};
-    size_t at[3] = {0, 0, 0};
-    bool copy[3] = {false, false, false};
+    const void *ptr[3] = {};
+    int64_t ld[3] = {};
+    size_t at[3] = {};
+    bool copy[3] = {};
     Copies copies;
-    for (int i = 0; i < (GATED ? 3 : 2); ++i) {
-        copy[i] = !fits(in[i].ptr, in[i].ld * es);
-        if (copy[i]) at[i] = copies.add((size_t)kp * rows[i]);
-    }
-    char *buf = nullptr;
-    hipError_t e;
-    if (copies.used && (e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf)) != hipSuccess) return e;
-    const TileChoice c = choose(GATED, M, N, 1, kb);
-    uint32_t *ws = nullptr;
-    if (c.ws_bytes && (e = workspace_get(stream, c.ws_bytes, WS_GEMM, (void **)&ws)) != hipSuccess) return e;
-    const void *ptr[3];
-    int64_t ld[3], bytes[3];
-    for (int i = 0; i < (GATED ? 3 : 2); ++i) {
+    for (int i = 0; i < OPERANDS; ++i) {
         ptr[i] = in[i].ptr;
         ld[i] = in[i].ld * es;
-        if (copy[i]) {
-            if ((e = pack_rows(in[i].ptr, ld[i], kb, buf + at[i], kp, rows[i], stream)) != hipSuccess) return e;
-            ptr[i] = buf + at[i];
-            ld[i] = kp;
-        }
-        bytes[i] = (rows[i] - 1) * ld[i] + kb;
+        copy[i] = !fits(ptr[i], ld[i]);
+        if (copy[i]) at[i] = copies.add((size_t)kp * rows[i]);
+    }
+    const Choice c = choose(GATED, M, N, kb, (int64_t)copies.used, kp <= kMaxRowBytes);
+    const bool tiled = c.form >= ROWS_FORMS;
+    char *buf = nullptr;
+    uint32_t *ws = nullptr;
+    hipError_t e = hipSuccess;
+    if (tiled && copies.used) e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf);
+    if (e == hipSuccess && tiled && c.tiling.ws_bytes) e = workspace_get(stream, c.tiling.ws_bytes, WS_GEMM, (void **)&ws);
+    if (e != hipSuccess) return e;
+    for (int i = 0; i < OPERANDS; ++i) {
+        if (!tiled || !copy[i]) continue;
+        if ((e = pack_rows(ptr[i], ld[i], kb, buf + at[i], kp, rows[i], stream)) != hipSuccess) return e;
+        ptr[i] = buf + at[i];
+        ld[i] = kp;
     }
     p.A[0] = p.A[1] = ptr[0];
     p.lda = ld[0];
-    p.a_bytes = bytes[0];
+    p.a_bytes = (M - 1) * ld[0] + kb;
     for (int h = 0; h < 2; ++h) {
         const int i = GATED ? 1 + h : 1;
         p.B[h] = ptr[i];
         p.ldb[h] = ld[i];
-        p.b_bytes[h] = bytes[i];
+        p.b_bytes[h] = (N - 1) * ld[i] + kb;
     }
     p.k_bytes = kb;
     p.M = M;
     p.N = N;
-    p.batch = 1;
-    p.part_steps = 0x7fffffff;
-    return run_product<ET, GATED, ALONG_K, ALONG_K>(p, c, ws, K, stream);
+    if (!tiled) return run_rows<ET, GATED>(p, c.form, K, stream);
+    return run_tiles<ET, GATED>(tiled_product(p, c.tiling, ws), c.form - ROWS_FORMS, K, stream);
+}
+
+// The two products of the gradient in one launch.  The workgroups are shared out by the steps there are to do; a product that
+// is not wanted has no tiles.
+template <int ET> hipError_t run_two(const Product &px, const Product &pw, const Tiling *c, int tile, int M, int N, int K, hipStream_t stream) {
+    const int64_t nx = c[0].count(), nw = c[1].count();
+    if (nx > 0x3fffffff || nw > 0x3fffffff) return hipErrorNotSupported;
+    hipError_t e = with_tile<ET, false, ALONG_K, ACROSS_K>(tile, [&](auto cfg) {
+        typedef decltype(cfg) Cfg0;
+        typedef TileCfg<ET, Cfg0::BM, Cfg0::BN, Cfg0::WM, Cfg0::WN, Cfg0::S, false, ACROSS_K, ACROSS_K> Cfg1;
+        const double wx = (double)nx * c[0].steps_per_split, ww = (double)nw * c[1].steps_per_split;
+        int64_t grid = nx + nw < resident<Cfg0>() ? nx + nw : resident<Cfg0>();
+        int64_t blocks = nx + nw <= grid ? nx : (int64_t)(grid * wx / (wx + ww) + 0.5);
+        if (nx && blocks < 1) blocks = 1;
+        if (nw && blocks > grid - 1) blocks = grid - 1;
+        if (blocks > nx) blocks = nx;
+        if (grid - blocks > nw) grid = blocks + nw;
+        auto kernel = two_tiles_kernel<Cfg0, Cfg1>;
+        hipError_t e = ensure_dynamic_lds((const void *)kernel, Cfg0::LDS);
+        if (e == hipSuccess) e = launch_kernel(kernel, dim3((unsigned)grid), dim3(Cfg0::THREADS), Cfg0::LDS, stream, ProductPair{{px, pw}}, (int)blocks);
+        return launched("ffn_two_tiles_kernel", type_letter(ET), Cfg0::BM, Cfg0::BN, Cfg0::THREADS, M, N, K, (unsigned)grid, 1, c[0].splits, e);
+    });
+    if (e != hipSuccess || (px.splits <= 1 && pw.splits <= 1)) return e;
+    const unsigned gx = px.splits > 1 ? join_grid(px) : 0, gw = pw.splits > 1 ? join_grid(pw) : 0;
+    const dim3 grid(gx > gw ? gx : gw, 2);
+    e = launch_kernel(join_two_kernel<ET>, grid, dim3(256), 0, stream, ProductPair{{px, pw}});
+    return launched("ffn_join_two_kernel", type_letter(ET), 1, 4, 256, M, N, K, grid.x, 2, px.splits > pw.splits ? px.splits : pw.splits, e);
 }
 
 template <int ET, int OT>
@@ -405,11 +491,35 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         copy[i] = used[i] && !fits(in[i].ptr, in[i].ld * 2);
         if (copy[i]) at[i] = copies.add((size_t)rows[i] * ld_copy);
     }
-    const TileChoice cx = choose(false, M, K, 1, row), cw = choose(false, N, K, 2, (int64_t)M * 2);
-    size_t sums = want_x ? cx.ws_bytes : 0;
-    if (want_w && cw.ws_bytes > sums) sums = cw.ws_bytes;
+    // One tile for both products; each cut into ranges of its depth as the model finds best.
+    int tile = 0;
+    Tiling c[2];
+    double best = 1e30;
+    for (int i = 0; i < TILE_FORMS; ++i) {
+        if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
+        for (int sx : kSplits) {
+            for (int sw : kSplits) {
+                const int fs = knobs().ffn_splits;
+                Tiling t[2];
+                if (want_x) t[0] = tiling(i, false, M, K, 1, row, fs ? fs : sx);
+                if (want_w) t[1] = tiling(i, false, N, K, 2, (int64_t)M * 2, fs ? fs : sw);
+                if (!fs && want_w && t[1].splits != sw) break;
+                if (!fs && want_x && t[0].splits != sx) break;
+                const double cost = tiled_cost(i, t, 2);
+                if (cost < best) {
+                    best = cost;
+                    tile = i;
+                    c[0] = t[0];
+                    c[1] = t[1];
+                }
+                if (fs || !want_w) break;
+            }
+            if (knobs().ffn_splits || !want_x) break;
+        }
+    }
     char *buf = nullptr;
     uint32_t *ws = nullptr;
+    const size_t sums_x = (size_t)round_up((int64_t)c[0].ws_bytes, 256), sums = sums_x + c[1].ws_bytes;
     hipError_t e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf);
     if (e == hipSuccess && sums) e = workspace_get(stream, sums, WS_GEMM, (void **)&ws);
     if (e != hipSuccess) return e;
@@ -425,46 +535,40 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     const unsigned grid = (unsigned)(ceil_div(work, 256) < 8192 ? ceil_div(work, 256) : 8192);
     e = launch_kernel(gate_grad_kernel<OT>, dim3(grid), dim3(256), 0, stream, dH.ptr, dH.ld, G.ptr, G.ld, U.ptr, U.ld, M, N, gate, (void *)grads, half);
     if ((e = launched("ffn_gate_grad_kernel", type_letter(ET), 1, 8, 256, M, N, K, grid, 1, 1, e)) != hipSuccess) return e;
-    Product p = {};
-    p.out_type = OT;
-    p.lda = row;
-    if (want_x) {  // [dG | dU] (M x 2 half) times [Wg; Wu]: the depth runs through Wg's rows, then through Wu's
-        p.A[0] = p.A[1] = grads;
-        p.a_bytes = M * row;
-        for (int h = 0; h < 2; ++h) {
-            p.B[h] = ptr[1 + h];
-            p.ldb[h] = ld[1 + h];
-            p.b_bytes[h] = (N - 1) * ld[1 + h] + (int64_t)K * 2;
-        }
-        p.k_bytes = row;
-        p.part_steps = (int)(half / 64);
-        p.C[0] = p.C[1] = dX.ptr;
-        p.ldc[0] = p.ldc[1] = dX.ld;
-        p.M = M;
-        p.N = K;
-        p.batch = 1;
-        if ((e = run_product<ET, false, ALONG_K, ACROSS_K>(p, cx, ws, (int)(2 * half), stream)) != hipSuccess) return e;
+    Product p[2] = {};  // [dG | dU] (M x 2 half) times [Wg; Wu]: the depth runs through Wg's rows, then through Wu's
+    p[0].A[0] = p[0].A[1] = grads;
+    p[0].a_bytes = M * row;
+    for (int h = 0; h < 2; ++h) {
+        p[0].B[h] = ptr[1 + h];
+        p[0].ldb[h] = ld[1 + h];
+        p[0].b_bytes[h] = (N - 1) * ld[1 + h] + (int64_t)K * 2;
     }
-    if (want_w) {  // dG^T X and dU^T X: the depth runs through the tokens
-        for (int z = 0; z < 2; ++z) {
-            p.A[z] = grads + z * half * 2;
-            p.B[z] = ptr[0];
-            p.ldb[z] = ld[0];
-            p.b_bytes[z] = (M - 1) * ld[0] + (int64_t)K * 2;
-        }
-        p.a_bytes = M * row - half * 2;
-        p.k_bytes = (int64_t)M * 2;
-        p.part_steps = 0x7fffffff;
-        p.C[0] = dWg.ptr;
-        p.C[1] = dWu.ptr;
-        p.ldc[0] = dWg.ld;
-        p.ldc[1] = dWu.ld;
-        p.M = N;
-        p.N = K;
-        p.batch = 2;
-        if ((e = run_product<ET, false, ACROSS_K, ACROSS_K>(p, cw, ws, M, stream)) != hipSuccess) return e;
+    p[0].k_bytes = row;
+    p[0].part_steps = (int)(half / 64);
+    p[0].C[0] = p[0].C[1] = dX.ptr;
+    p[0].ldc[0] = p[0].ldc[1] = dX.ld;
+    p[0].M = M;
+    // dG^T X and dU^T X: the depth runs through the tokens
+    for (int z = 0; z < 2; ++z) {
+        p[1].A[z] = grads + z * half * 2;
+        p[1].B[z] = ptr[0];
+        p[1].ldb[z] = ld[0];
+        p[1].b_bytes[z] = (M - 1) * ld[0] + (int64_t)K * 2;
     }
-    return hipSuccess;
+    p[1].a_bytes = M * row - half * 2;
+    p[1].k_bytes = (int64_t)M * 2;
+    p[1].C[0] = dWg.ptr;
+    p[1].C[1] = dWu.ptr;
+    p[1].ldc[0] = dWg.ld;
+    p[1].ldc[1] = dWu.ld;
+    p[1].M = N;
+    for (int i = 0; i < 2; ++i) {
+        p[i].out_type = OT;
+        p[i].lda = row;
+        p[i].N = K;
+        p[i] = tiled_product(p[i], c[i], i ? ws + sums_x / 4 : ws);
+    }
+    return run_two<ET>(p[0], p[1], c, tile, M, N, K, stream);
 }
 
 }  // namespace

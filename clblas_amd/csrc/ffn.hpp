@@ -35,6 +35,10 @@ struct Product {
     int64_t ws_ld, ws_plane, ws_split;
 };
 
+struct ProductPair {
+    Product p[2];
+};
+
 // A matrix as the caller gave it: rows of `ld` elements.
 struct Mat {
     const void *ptr = nullptr;
@@ -44,6 +48,9 @@ struct OutMat {
     void *ptr = nullptr;
     int64_t ld = 0;
 };
+
+// Rows of a tiled operand are addressed across a tile with 32-bit offsets: at most this many bytes from row to row.
+constexpr int64_t kMaxRowBytes = ((int64_t)1 << 22) - 1024;
 
 hipError_t quantize_rows(int type, int M, int K, Mat X, int8_t *Q, int64_t ldq, float *scale, hipStream_t stream);
 // C = A B^T (8-bit, scaled), or with Bu: act(A Bg^T) o (A Bu^T).

@@ -589,8 +589,11 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     TileAt t = tile_at<Cfg>(fresh(args), id);
     CBA_FFN_WAIT_VM((S - 1) * (LA + LB));
     publish(lds, t.bytes(0));
+    auto read_first = [&](const char *at) {
 #pragma unroll
-    for (int i = 0; i < TM + TN; ++i) read_one(lds, 0, i);
+        for (int i = 0; i < TM + TN; ++i) read_one(at, 0, i);
+    };
+    read_first(lds);
 
     // MFMAs kk of a step.  Loads and reads are spread between their rows: behind the first, whose operands are there, and
     // none behind the last.
@@ -662,23 +665,31 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
         if (next_id >= end) break;
         id = next_id;
         t = tile_at<Cfg>(fresh(args), id);
-        // (read once more: kept over the stores, these registers would be spilled)
-#pragma unroll
-        for (int i = 0; i < TM + TN; ++i) read_one(stage, 0, i);
+        read_first(stage);  // (once more: kept over the stores, these registers would be spilled)
     }
     CBA_FFN_WAIT_VM(0);  // (nothing may be on its way into LDS when the workgroup ends)
 }
 
 // Workgroups are handed to the 8 XCDs in turn, and each XCD has an L2 of its own: every XCD walks a contiguous piece of the
-// list, its workgroups side by side.
-template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void tile_kernel(Product p) {
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const int total = p.tiles_m * p.tiles_n * p.batch * p.splits;
-    const int xcds = gridDim.x < 8 ? gridDim.x : 8, xcd = blockIdx.x % xcds, place = blockIdx.x / xcds;
+// list, its workgroups side by side.  This is workgroup `block` of the `blocks` that walk this list.
+template <typename Cfg> static __device__ __forceinline__ void walk_list(Args *p, int block, int blocks, char *lds) {
+    const int total = p->tiles_m * p->tiles_n * p->batch * p->splits;
+    const int xcds = blocks < 8 ? blocks : 8, xcd = block % xcds, place = block / xcds;
     const int per = total / xcds, rem = total % xcds;
     const int first = xcd * per + (xcd < rem ? xcd : rem), end = first + per + (xcd < rem ? 1 : 0);
-    const int stride = (gridDim.x - xcd + xcds - 1) / xcds;  // workgroups on this XCD
-    walk_tiles<Cfg>(kernel_args(), first + place, stride, end, lds);
+    const int stride = (blocks - xcd + xcds - 1) / xcds;  // workgroups on this XCD
+    walk_tiles<Cfg>(p, first + place, stride, end, lds);
+}
+template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void tile_kernel(Product) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    walk_list<Cfg>(kernel_args(), blockIdx.x, gridDim.x, lds);
+}
+// Two products in one launch (both sides of the gradient): the first `blocks` workgroups walk the first one's tiles.
+template <typename Cfg0, typename Cfg1> __global__ __launch_bounds__(Cfg0::THREADS, 2) void two_tiles_kernel(ProductPair, int blocks) {
+    static_assert(Cfg0::THREADS == Cfg1::THREADS && Cfg0::LDS == Cfg1::LDS, "");
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    if ((int)blockIdx.x < blocks) walk_list<Cfg0>(kernel_args(), blockIdx.x, blocks, lds);
+    else walk_list<Cfg1>(kernel_args() + 1, blockIdx.x - blocks, gridDim.x - blocks, lds);
 }
 
 // ---- the product from registers ----
@@ -835,7 +846,8 @@ template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void rows_
 // Adds up the depth ranges of a split product (in their order, whatever finished first) and finishes the results.
 // Partial sums: [range][plane][row][column], rows of ws_ld (a multiple of 4) 32-bit sums; planes are the batch's
 // entries or the gate's two products.
-template <int ET, bool GATED> __global__ __launch_bounds__(256) void join_kernel(Product p) {
+template <int ET, bool GATED> static __device__ __forceinline__ void join(Args *args) {
+    Args &p = *args;
     const int64_t per_row = p.ws_ld >> 2, per_plane = per_row * p.M, total = per_plane * p.batch;
     typedef typename ElemOf<ET>::Acc S;
     typedef S sx4 __attribute__((ext_vector_type(4)));
@@ -850,10 +862,15 @@ template <int ET, bool GATED> __global__ __launch_bounds__(256) void join_kernel
             a += *reinterpret_cast<const sx4 *>(w);
             if (GATED) b += *reinterpret_cast<const sx4 *>(w + p.ws_plane);
         }
-        float x[4] = {(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
-        float y[4] = {(float)b[0], (float)b[1], (float)b[2], (float)b[3]};
-        finish4<ET, GATED>(*kernel_args(), z, m, n, x, y);
+        const float x[4] = {(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
+        const float y[4] = {(float)b[0], (float)b[1], (float)b[2], (float)b[3]};
+        finish4<ET, GATED>(p, z, m, n, x, y);
     }
+}
+template <int ET, bool GATED> __global__ __launch_bounds__(256) void join_kernel(Product) { join<ET, GATED>(kernel_args()); }
+template <int ET> __global__ __launch_bounds__(256) void join_two_kernel(ProductPair) {
+    Args *p = kernel_args() + blockIdx.y;
+    if (p->splits > 1) join<ET, false>(p);
 }
 
 }  // namespace ffn
