@@ -444,39 +444,61 @@ def hemm(prefix, order, side, uplo, M, N, alpha, A, offA, lda, B, offB, ldb, bet
 
 
 # ---- the products of a gated feed-forward layer (row-major; include/clblas_amd.h) ----
+# (Calls of a few microseconds: addresses go to ctypes as plain integers.)
+
+def _addr(x):
+    return x if x is None or isinstance(x, int) else x.data_ptr()
+
+
+_raw_stream = None
+
+
+def _stream_addr(stream, x):
+    """The stream's handle (None: torch's current one on the current device, where tensor x has to live)."""
+    global _raw_stream
+    if stream is None:
+        import torch
+        device = torch.cuda.current_device()
+        if isinstance(x, torch.Tensor) and x.get_device() != device:
+            raise ValueError("matrix on %s, but the current device is cuda:%d" % (x.device, device))
+        if _raw_stream is None:  # (current_stream() builds a Stream object: 2.6 us, as long as a launch)
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return _raw_stream(device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
 
 def quantize_rows(type_, M, K, X, offX, ldx, Q, offQ, ldq, scale, stream=None):
     """clblasAmdQuantizeRows: rows of X (Type) to 8-bit integers Q with one scale each."""
-    return load_library().clblasAmdQuantizeRows(int(type_), M, K, _ptr(X), offX, ldx, _ptr(Q), offQ, ldq, _ptr(scale),
-                                                _stream(stream))
+    return load_library().clblasAmdQuantizeRows(int(type_), M, K, _addr(X), offX, ldx, _addr(Q), offQ, ldq, _addr(scale),
+                                                _stream_addr(stream, X))
 
 
 def i8gemm(typeC, M, N, K, A, offA, lda, scaleA, B, offB, ldb, scaleB, C, offC, ldc, stream=None):
     """clblasAmdI8gemm: C = diag(scaleA) A B^T diag(scaleB), A and B 8-bit, C of typeC (Type)."""
-    return load_library().clblasAmdI8gemm(int(typeC), M, N, K, _ptr(A), offA, lda, _ptr(scaleA), _ptr(B), offB, ldb,
-                                          _ptr(scaleB), _ptr(C), offC, ldc, _stream(stream))
+    return load_library().clblasAmdI8gemm(int(typeC), M, N, K, _addr(A), offA, lda, _addr(scaleA), _addr(B), offB, ldb,
+                                          _addr(scaleB), _addr(C), offC, ldc, _stream_addr(stream, A))
 
 
 def gated(type_, gate, M, N, K, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, H, offH, ldh, G=None, offG=0, ldg=0,
           U=None, offU=0, ldu=0, stream=None):
     """clblasAmdGated: H = act(X Wg^T) o (X Wu^T); G and U (both or neither) receive the two products."""
-    return load_library().clblasAmdGated(int(type_), int(gate), M, N, K, _ptr(X), offX, ldx, _ptr(Wg), offWg, ldwg,
-                                         _ptr(Wu), offWu, ldwu, _ptr(H), offH, ldh, _ptr(G), offG, ldg, _ptr(U), offU,
-                                         ldu, _stream(stream))
+    return load_library().clblasAmdGated(int(type_), int(gate), M, N, K, _addr(X), offX, ldx, _addr(Wg), offWg, ldwg,
+                                         _addr(Wu), offWu, ldwu, _addr(H), offH, ldh, _addr(G), offG, ldg, _addr(U), offU,
+                                         ldu, _stream_addr(stream, X))
 
 
 def gated_i8(typeH, gate, M, N, K, X, offX, ldx, scaleX, Wg, offWg, ldwg, scaleWg, Wu, offWu, ldwu, scaleWu, H, offH,
              ldh, stream=None):
     """clblasAmdGatedI8: the gated product on 8-bit operands with scales, H of typeH (Type)."""
-    return load_library().clblasAmdGatedI8(int(typeH), int(gate), M, N, K, _ptr(X), offX, ldx, _ptr(scaleX), _ptr(Wg),
-                                           offWg, ldwg, _ptr(scaleWg), _ptr(Wu), offWu, ldwu, _ptr(scaleWu), _ptr(H),
-                                           offH, ldh, _stream(stream))
+    return load_library().clblasAmdGatedI8(int(typeH), int(gate), M, N, K, _addr(X), offX, ldx, _addr(scaleX), _addr(Wg),
+                                           offWg, ldwg, _addr(scaleWg), _addr(Wu), offWu, ldwu, _addr(scaleWu), _addr(H),
+                                           offH, ldh, _stream_addr(stream, X))
 
 
 def gated_grad(type_, gate, M, N, K, dH, offdH, lddh, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, G, offG, ldg, U,
                offU, ldu, dX, offdX, lddx, dWg, offdWg, lddwg, dWu, offdWu, lddwu, stream=None):
     """clblasAmdGatedGrad: dX (or None), dWg and dWu (or both None) from dH, the operands and the stored G and U."""
-    return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, _ptr(dH), offdH, lddh, _ptr(X), offX, ldx,
-                                             _ptr(Wg), offWg, ldwg, _ptr(Wu), offWu, ldwu, _ptr(G), offG, ldg, _ptr(U),
-                                             offU, ldu, _ptr(dX), offdX, lddx, _ptr(dWg), offdWg, lddwg, _ptr(dWu),
-                                             offdWu, lddwu, _stream(stream))
+    return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, _addr(dH), offdH, lddh, _addr(X), offX, ldx,
+                                             _addr(Wg), offWg, ldwg, _addr(Wu), offWu, ldwu, _addr(G), offG, ldg, _addr(U),
+                                             offU, ldu, _addr(dX), offdX, lddx, _addr(dWg), offdWg, lddwg, _addr(dWu),
+                                             offdWu, lddwu, _stream_addr(stream, X))

@@ -200,12 +200,11 @@ char type_letter(int et) { return et == ET_I8 ? 'i' : et == ET_F16 ? 'h' : 'b'; 
 struct RowsShape { int tm, tn; };
 const RowsShape kRows[] = {{1, 1}, {2, 1}, {2, 2}, {4, 2}};
 enum { ROWS_FORMS = 4, TILE_FORMS = 5 };
-// step: us per step of 128 bytes of depth, alone on a CU / per tile where more tiles than CUs keep it busy; per_cu: workgroups
-// that a CU holds.  Measured on products of 128 ... 8192 rows, 1024 ... 12288 channels, 1024 ... 8192 deep (alone: e.g. 64 x 64
+// step: us per step of 128 bytes of depth, alone on a CU / per tile where more tiles than CUs keep it busy.  Measured on products of 128 ... 8192 rows, 1024 ... 12288 channels, 1024 ... 8192 deep (alone: e.g. 64 x 64
 // at 256 x 1024 x 4096 8-bit, 32 steps in 14.9 us; busy: 64 x 128 at 1024 x 4096 x 4096 gated, 4 x 64 steps per CU in 102 us).
-struct TileShape { int bm, bn, per_cu; double step_alone, step_busy; };
+struct TileShape { int log_bm, log_bn; double step_alone, step_busy; };
 const TileShape kTiles[TILE_FORMS] = {
-    {256, 256, 1, 1.50, 1.62}, {256, 128, 1, 0.87, 0.97}, {128, 128, 2, 0.97, 0.57}, {64, 128, 2, 0.50, 0.375}, {64, 64, 2, 0.36, 0.27}};
+    {8, 8, 1.50, 1.62}, {8, 7, 0.87, 0.97}, {7, 7, 0.97, 0.57}, {6, 7, 0.50, 0.375}, {6, 6, 0.36, 0.27}};  // (edges: powers of two)
 
 template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
     switch (tile) {
@@ -224,23 +223,29 @@ struct Tiling {
     size_t ws_bytes = 0;
     int64_t count() const { return (int64_t)tiles_m * tiles_n * batch * splits; }
 };
-Tiling tiling(int tile, bool gated, int M, int N, int batch, int64_t k_bytes, int splits) {
+uint32_t blocks_of(uint32_t n, int shift) { return (n + (1u << shift) - 1) >> shift; }
+// (This and what follows runs in every call: powers of two and 32-bit quotients.)
+Tiling tiling(int tile, bool gated, int M, int N, int batch, int64_t k_bytes) {
     Tiling c;
     const TileShape &t = kTiles[tile];
-    const int64_t steps = ceil_div(k_bytes, 128);
-    c.tiles_m = (int)ceil_div(M, t.bm);
-    c.tiles_n = (int)ceil_div(N, gated ? t.bn / 2 : t.bn);
+    c.tiles_m = (int)blocks_of(M, t.log_bm);
+    c.tiles_n = (int)blocks_of(N, gated ? t.log_bn - 1 : t.log_bn);
     c.batch = batch;
-    if (splits > steps) splits = (int)steps;
-    if (splits < 1 || t.bm * t.bn >= 65536) splits = 1;  // (the largest tiles do not split: TileCfg::SPLITS)
-    c.steps_per_split = (int)ceil_div(steps, splits);
-    c.splits = (int)ceil_div(steps, c.steps_per_split);
-    if (c.splits > 1) {
-        c.ws_ld = round_up(N, 4);
-        c.ws_plane = c.ws_ld * M;
-        c.ws_split = c.ws_plane * (gated ? 2 : batch);
-        c.ws_bytes = (size_t)c.ws_split * 4 * c.splits;
-    }
+    c.steps_per_split = (int)((k_bytes + 127) >> 7);
+    return c;
+}
+// Cuts the depth into `splits` ranges at most.  (The largest tiles do not split: TileCfg::SPLITS.)
+Tiling cut_depth(Tiling c, int tile, bool gated, int M, int N, int splits) {
+    const uint32_t steps = (uint32_t)c.steps_per_split;
+    if (splits <= 1 || steps <= 1 || tile == 0) return c;
+    if ((uint32_t)splits > steps) splits = (int)steps;
+    c.steps_per_split = (int)((steps + splits - 1) / (uint32_t)splits);
+    c.splits = (int)((steps + c.steps_per_split - 1) / (uint32_t)c.steps_per_split);
+    if (c.splits == 1) return c;
+    c.ws_ld = ((int64_t)N + 3) & ~(int64_t)3;
+    c.ws_plane = c.ws_ld * M;
+    c.ws_split = c.ws_plane * (gated ? 2 : c.batch);
+    c.ws_bytes = (size_t)c.ws_split * 4 * c.splits;
     return c;
 }
 
@@ -258,7 +263,7 @@ double tiled_cost(int tile, const Tiling *c, int n) {
     }
     double time;
     if (count <= 256) time = longest * t.step_alone;
-    else if (n == 1) time = (double)ceil_div((int64_t)count, 256) * longest * t.step_busy;
+    else if (n == 1) time = (double)(((int64_t)count + 255) >> 8) * longest * t.step_busy;
     else time = (steps / 256 > longest ? steps / 256 : longest) * t.step_busy;
     return 4.5 + time + (partial > 0 ? 3.0 + partial * 0.6e-6 : 0.0);
 }
@@ -297,10 +302,12 @@ Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool ti
     if (!tiled) return best;
     for (int i = 0; i < TILE_FORMS; ++i) {
         if (forced >= 0 && forced != ROWS_FORMS + i) continue;
+        const Tiling whole = tiling(i, gated, M, N, 1, k_bytes);
         for (int splits : kSplits) {
-            if (knobs().ffn_splits && splits != 1) break;
-            const Tiling t = tiling(i, gated, M, N, 1, k_bytes, knobs().ffn_splits ? knobs().ffn_splits : splits);
-            if (t.splits != splits && !knobs().ffn_splits) break;
+            const int fs = knobs().ffn_splits;
+            if (splits > 1 && (fs || whole.count() * splits > 512)) break;  // (more only costs)
+            const Tiling t = cut_depth(whole, i, gated, M, N, fs ? fs : splits);
+            if (!fs && t.splits != splits) break;
             const double cost = tiled_cost(i, &t, 1) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
             if (cost < best.cost || (forced >= 0 && best.form != forced)) {
                 best.form = ROWS_FORMS + i;
@@ -497,24 +504,24 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     double best = 1e30;
     for (int i = 0; i < TILE_FORMS; ++i) {
         if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
-        for (int sx : kSplits) {
-            for (int sw : kSplits) {
-                const int fs = knobs().ffn_splits;
-                Tiling t[2];
-                if (want_x) t[0] = tiling(i, false, M, K, 1, row, fs ? fs : sx);
-                if (want_w) t[1] = tiling(i, false, N, K, 2, (int64_t)M * 2, fs ? fs : sw);
-                if (!fs && want_w && t[1].splits != sw) break;
-                if (!fs && want_x && t[0].splits != sx) break;
-                const double cost = tiled_cost(i, t, 2);
-                if (cost < best) {
-                    best = cost;
-                    tile = i;
-                    c[0] = t[0];
-                    c[1] = t[1];
-                }
-                if (fs || !want_w) break;
+        Tiling whole[2];
+        if (want_x) whole[0] = tiling(i, false, M, K, 1, row);
+        if (want_w) whole[1] = tiling(i, false, N, K, 2, (int64_t)M * 2);
+        const int longest = whole[0].steps_per_split > whole[1].steps_per_split ? whole[0].steps_per_split : whole[1].steps_per_split;
+        for (int cut : kSplits) {  // into ranges of about the same length for both
+            const int fs = knobs().ffn_splits;
+            if (cut > 1 && (fs || cut > longest || whole[0].count() + whole[1].count() > 512)) break;
+            const uint32_t range = (uint32_t)(longest + cut - 1) / (uint32_t)cut;
+            Tiling t[2];
+            for (int j = 0; j < 2; ++j) t[j] = cut_depth(whole[j], i, false, j ? N : M, K, fs ? fs : (int)((whole[j].steps_per_split + range - 1) / range));
+            if (cut > 1 && t[0].count() + t[1].count() > 512) break;
+            const double cost = tiled_cost(i, t, 2);
+            if (cost < best) {
+                best = cost;
+                tile = i;
+                c[0] = t[0];
+                c[1] = t[1];
             }
-            if (knobs().ffn_splits || !want_x) break;
         }
     }
     char *buf = nullptr;
