@@ -103,21 +103,31 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(con
 
 // ---- copies that make an operand fit the tiled product ----
 
-// Rows of `bytes` bytes, `ld` apart and aligned to nothing -> rows `ld_to` apart (a multiple of 16), zeros behind.
-__global__ __launch_bounds__(256) void pack_rows_kernel(const char *from, int64_t ld, int64_t bytes, char *to, int64_t ld_to, int64_t rows) {
-    const int64_t per = ld_to >> 4, total = per * rows;
+// Rows of `bytes` bytes, `ld` apart and aligned to nothing -> rows `ld_to` apart (a multiple of 16), zeros behind.  One launch
+// for all operands of a product.
+struct Copy {
+    const char *from;
+    char *to;
+    int64_t ld, bytes, ld_to, rows;
+};
+struct CopyList {
+    Copy c[3];
+};
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyList list) {
+    const Copy &c = list.c[blockIdx.y];
+    const int64_t per = c.ld_to >> 4, total = per * c.rows;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
         const int64_t row = t / per, at = (t - row * per) * 16;
-        const char *src = from + row * ld + at;
+        const char *src = c.from + row * c.ld + at;
         char v[16] = {};
-        if (at + 16 <= bytes) {
+        if (at + 16 <= c.bytes) {
             __builtin_memcpy(v, src, 16);
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                if (at + e < bytes) v[e] = src[e];
+                if (at + e < c.bytes) v[e] = src[e];
         }
-        __builtin_memcpy(__builtin_assume_aligned(to + row * ld_to + at, 16), v, 16);
+        __builtin_memcpy(__builtin_assume_aligned(c.to + row * c.ld_to + at, 16), v, 16);
     }
 }
 
@@ -252,7 +262,9 @@ Tiling cut_depth(Tiling c, int tile, bool gated, int M, int N, int splits) {
 // Time (us) of a launch over tilings that share it: the steps that the busiest of 256 CUs goes through, about 4.5 us for the
 // launch, the first loads and the results, and for sums in pieces a second launch (3 us) and the partial sums, written and
 // read again, at 0.6 us per MB (256 x 4096 x 4096 gated in two ranges of 64 x 128 tiles: 16.8 MB, 43.5 us; in one, 36.7).
-double tiled_cost(int tile, const Tiling *c, int n) {
+// memory: us that the operands take from memory.  Tilings that share a launch share the CUs: then a workgroup's own steps take as
+// long as its CU needs for one of each of its workgroups (the deepest tiles end last).
+double tiled_cost(int tile, const Tiling *c, int n, double memory) {
     const TileShape &t = kTiles[tile];
     double count = 0, steps = 0, longest = 0, partial = 0;
     for (int i = 0; i < n; ++i) {
@@ -264,7 +276,11 @@ double tiled_cost(int tile, const Tiling *c, int n) {
     double time;
     if (count <= 256) time = longest * t.step_alone;
     else if (n == 1) time = (double)(((int64_t)count + 255) >> 8) * longest * t.step_busy;
-    else time = (steps / 256 > longest ? steps / 256 : longest) * t.step_busy;
+    else {
+        const double own = longest * (t.log_bm + t.log_bn <= 14 ? 2 : 1) * t.step_busy, all = steps / 256 * t.step_busy;
+        time = own > all ? own : all;
+    }
+    if (time < memory) time = memory;
     return 4.5 + time + (partial > 0 ? 3.0 + partial * 0.6e-6 : 0.0);
 }
 
@@ -279,11 +295,10 @@ struct Choice {
 
 // From registers: what the busiest CU reads, at 33 bytes per ns (measured for workgroups of 16 x 16 ... 64 x 32 results,
 // gated and 8-bit, 16 ... 256 rows; within 10 %), or the weights from memory at 5.4 TB/s; 2.8 us for the launch.
-double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes) {
+double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes, double memory) {
     const int64_t groups = ceil_div(M, 16 * s.tm) * ceil_div(N, 16 * s.tn);
     const int64_t rows = (M < 16 * s.tm ? M : 16 * s.tm) + 16 * s.tn * (gated ? 2 : 1);
     const double cu = (double)ceil_div(groups, 256) * rows * k_bytes / 33e3;
-    const double memory = ((double)M + (double)N * (gated ? 2 : 1)) * k_bytes / 5.4e6;
     return 2.8 + (cu > memory ? cu : memory);
 }
 
@@ -291,9 +306,10 @@ double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes) 
 // anything as it is.  tiled: whether the rows are short enough for the tiled forms.
 Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool tiled) {
     Choice best;
+    const double memory = ((double)M + (double)N * (gated ? 2 : 1)) * k_bytes / 5.4e6;
     const int forced = knobs().ffn_form;
     for (int i = 0; i < ROWS_FORMS; ++i) {
-        const double cost = rows_cost(kRows[i], gated, M, N, k_bytes);
+        const double cost = rows_cost(kRows[i], gated, M, N, k_bytes, memory);
         if (forced >= 0 ? forced == i || (!tiled && i == 0) : cost < best.cost) {
             best.form = i;
             best.cost = cost;
@@ -308,7 +324,7 @@ Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool ti
             if (splits > 1 && (fs || whole.count() * splits > 512)) break;  // (more only costs)
             const Tiling t = cut_depth(whole, i, gated, M, N, fs ? fs : splits);
             if (!fs && t.splits != splits) break;
-            const double cost = tiled_cost(i, &t, 1) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
+            const double cost = tiled_cost(i, &t, 1, memory) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
             if (cost < best.cost || (forced >= 0 && best.form != forced)) {
                 best.form = ROWS_FORMS + i;
                 best.tiling = t;
@@ -399,18 +415,20 @@ bool fits(const void *ptr, int64_t ld_bytes) {
     return (reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && (ld_bytes & 3) == 0 && ld_bytes <= kMaxRowBytes;
 }
 
-hipError_t pack_rows(const void *from, int64_t ld, int64_t bytes, char *to, int64_t ld_to, int64_t rows, hipStream_t stream) {
-    const int64_t work = (ld_to >> 4) * rows;
-    const unsigned grid = (unsigned)(ceil_div(work, 256) < 4096 ? ceil_div(work, 256) : 4096);
-    hipError_t e = launch_kernel(pack_rows_kernel, dim3(grid), dim3(256), 0, stream, (const char *)from, ld, bytes, to, ld_to, rows);
-    return launched("ffn_pack_rows_kernel", 'p', 1, 16, 256, (int)rows, (int)bytes, 0, grid, 1, 1, e);
+hipError_t copy_rows(const CopyList &list, int n, hipStream_t stream) {
+    if (n == 0) return hipSuccess;
+    int64_t work = 0;
+    for (int i = 0; i < n; ++i) work = list.c[i].rows * (list.c[i].ld_to >> 4) > work ? list.c[i].rows * (list.c[i].ld_to >> 4) : work;
+    const dim3 grid((unsigned)(ceil_div(work, 256) < 4096 ? ceil_div(work, 256) : 4096), (unsigned)n);
+    hipError_t e = launch_kernel(copy_rows_kernel, grid, dim3(256), 0, stream, list);
+    return launched("ffn_copy_rows_kernel", 'p', 1, 16, 256, (int)list.c[0].rows, (int)list.c[0].bytes, 0, grid.x, grid.y, 1, e);
 }
 
 // A product whose operands are the caller's: chooses its form, copies what that form cannot load, and runs it.
 template <int ET, bool GATED>
 hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Product p, hipStream_t stream) {
     constexpr int OPERANDS = GATED ? 3 : 2;
-    const int64_t kb = (int64_t)K * es, kp = round_up(kb, 16);
+    const int64_t kb = (int64_t)K * es, kp = round_up(kb, 128);  // (copies: rows of whole cache lines)
     const Mat in[3] = {A, B0, B1};
     const int64_t rows[3] = {M, N, N};
     const void *ptr[3] = {};
@@ -432,12 +450,15 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
     if (tiled && copies.used) e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf);
     if (e == hipSuccess && tiled && c.tiling.ws_bytes) e = workspace_get(stream, c.tiling.ws_bytes, WS_GEMM, (void **)&ws);
     if (e != hipSuccess) return e;
+    CopyList list = {};
+    int n = 0;
     for (int i = 0; i < OPERANDS; ++i) {
         if (!tiled || !copy[i]) continue;
-        if ((e = pack_rows(ptr[i], ld[i], kb, buf + at[i], kp, rows[i], stream)) != hipSuccess) return e;
+        list.c[n++] = Copy{static_cast<const char *>(ptr[i]), buf + at[i], ld[i], kb, kp, rows[i]};
         ptr[i] = buf + at[i];
         ld[i] = kp;
     }
+    if ((e = copy_rows(list, n, stream)) != hipSuccess) return e;
     p.A[0] = p.A[1] = ptr[0];
     p.lda = ld[0];
     p.a_bytes = (M - 1) * ld[0] + kb;
@@ -488,7 +509,7 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     const bool want_x = dX.ptr, want_w = dWg.ptr;
     // operands that the tiles load as they are, or copies
     Mat in[3] = {X, Wg, Wu};
-    const int64_t rows[3] = {M, N, N}, ld_copy = round_up((int64_t)K * 2, 16);
+    const int64_t rows[3] = {M, N, N}, ld_copy = round_up((int64_t)K * 2, 128);
     const bool used[3] = {want_w, want_x, want_x};
     Copies copies;
     const size_t at_grads = copies.add((size_t)M * row);
@@ -510,12 +531,12 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         const int longest = whole[0].steps_per_split > whole[1].steps_per_split ? whole[0].steps_per_split : whole[1].steps_per_split;
         for (int cut : kSplits) {  // into ranges of about the same length for both
             const int fs = knobs().ffn_splits;
-            if (cut > 1 && (fs || cut > longest || whole[0].count() + whole[1].count() > 512)) break;
+            if (cut > 1 && (fs || cut > longest || whole[0].count() + whole[1].count() > 2048)) break;
             const uint32_t range = (uint32_t)(longest + cut - 1) / (uint32_t)cut;
             Tiling t[2];
             for (int j = 0; j < 2; ++j) t[j] = cut_depth(whole[j], i, false, j ? N : M, K, fs ? fs : (int)((whole[j].steps_per_split + range - 1) / range));
-            if (cut > 1 && t[0].count() + t[1].count() > 512) break;
-            const double cost = tiled_cost(i, t, 2);
+            if (cut > 1 && t[0].count() + t[1].count() > 2048) break;
+            const double cost = tiled_cost(i, t, 2, 0.0);
             if (cost < best) {
                 best = cost;
                 tile = i;
@@ -533,11 +554,14 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     char *grads = buf + at_grads;
     const void *ptr[3];
     int64_t ld[3];
+    CopyList list = {};
+    int n = 0;
     for (int i = 0; i < 3; ++i) {
         ptr[i] = copy[i] ? buf + at[i] : in[i].ptr;
         ld[i] = copy[i] ? ld_copy : in[i].ld * 2;
-        if (copy[i] && (e = pack_rows(in[i].ptr, in[i].ld * 2, (int64_t)K * 2, buf + at[i], ld_copy, rows[i], stream)) != hipSuccess) return e;
+        if (copy[i]) list.c[n++] = Copy{static_cast<const char *>(in[i].ptr), buf + at[i], in[i].ld * 2, (int64_t)K * 2, ld_copy, rows[i]};
     }
+    if ((e = copy_rows(list, n, stream)) != hipSuccess) return e;
     const int64_t work = M * (half / 8);
     const unsigned grid = (unsigned)(ceil_div(work, 256) < 8192 ? ceil_div(work, 256) : 8192);
     e = launch_kernel(gate_grad_kernel<OT>, dim3(grid), dim3(256), 0, stream, dH.ptr, dH.ld, G.ptr, G.ld, U.ptr, U.ld, M, N, gate, (void *)grads, half);

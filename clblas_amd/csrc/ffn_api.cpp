@@ -156,7 +156,7 @@ clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M
         CBA_CHECK(check_rows(N, K, lddwu, MAT_C, dWu, offdWu, 2));
     }
     if (M > kMaxDim || N > kMaxDim || K > kMaxDim ||
-        4 * (N + 63) > (size_t)cba::ffn::kMaxRowBytes || 2 * K + 15 > (size_t)cba::ffn::kMaxRowBytes ||  // rows of [dG | dU] and of copies
+        4 * (N + 63) > (size_t)cba::ffn::kMaxRowBytes || 2 * K + 127 > (size_t)cba::ffn::kMaxRowBytes ||  // rows of [dG | dU] and of copies
         !strides_in_range({lddh, ldx, ldwg, ldwu, ldg, ldu, dX ? lddx : 0, dWg ? lddwg : 0, dWg ? lddwu : 0}))
         return clblasNotImplemented;
     return map_hip_error(cba::with_workspaces_secured(stream, [&] {

@@ -68,10 +68,11 @@ static __device__ __forceinline__ float gate_value(int gate, float g) {
 // act(g) and act'(g).  The slope is flat (0 or 1 to the last bit) far from zero; |g| is cut off there, so that the
 // products in it cannot turn into 0 * inf.  NaN passes through the comparisons.
 static __device__ __forceinline__ void gate_value_and_slope(int gate, float g, float &value, float &slope) {
-    value = gate_value(gate, g);
     const float c = g > 128.f ? 128.f : (g < -128.f ? -128.f : g);
     if (gate == GATE_GELU) {
-        slope = 0.5f * erfcf(-0.70710678f * c) + c * 0.39894228f * __expf(-0.5f * c * c);
+        const float p = 0.5f * erfcf(-0.70710678f * c);
+        value = g * p;
+        slope = p + c * 0.39894228f * __expf(-0.5f * c * c);
         return;
     }
     float x = c, dx = 1.f;
@@ -80,6 +81,7 @@ static __device__ __forceinline__ void gate_value_and_slope(int gate, float g, f
         dx = 1.59576912f * (1.f + 0.134145f * c * c);
     }
     const float s = __builtin_amdgcn_rcpf(1.f + __expf(-x)), t = __builtin_amdgcn_rcpf(1.f + __expf(x));  // t = 1 - s
+    value = g * s;
     slope = s + c * s * t * dx;
 }
 
