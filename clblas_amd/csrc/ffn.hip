@@ -339,7 +339,7 @@ Product tiled_product(Product p, const Tiling &c, uint32_t *ws) {
     p.tiles_m = c.tiles_m;
     p.tiles_n = c.tiles_n;
     p.batch = c.batch;
-    p.group_m = 8;
+    p.group_m = 4;  // (8192 x 12288 x 4096 gated, us: 4 1287, 6 1365, 8 1308, 16 1342; 8-bit 8192^3 424, 424, 431, 444)
     p.splits = c.splits;
     p.steps_per_split = c.steps_per_split;
     p.ws = ws;

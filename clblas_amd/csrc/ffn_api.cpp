@@ -21,6 +21,15 @@ clblasStatus check_rows(size_t rows, size_t cols, size_t ld, MatId which, const 
     return check_matrix_sizes(clblasRowMajor, clblasNoTrans, rows, cols, ld, which, base, off, tsize);
 }
 
+// A vector of n floats (one per token: VecX, one per channel: VecY): with CLBLAS_AMD_CHECK_MEM=1 it has to fit behind its pointer.
+clblasStatus check_scales(const float *scale, size_t n, bool tokens) {
+    if (!cba::knobs().check_mem) return clblasSuccess;
+    const size_t mem = cba::mem_behind(scale);
+    if (mem == 0) return tokens ? clblasInvalidVecX : clblasInvalidVecY;
+    if (mem / sizeof(float) < n) return tokens ? clblasInsufficientMemVecX : clblasInsufficientMemVecY;
+    return clblasSuccess;
+}
+
 // Byte arithmetic on strides stays in 64 bits: rows * ld * size below 2^63 (no memory is that large, so whatever
 // passes this only has to be addressed correctly).
 bool strides_in_range(std::initializer_list<size_t> lds) {
@@ -63,6 +72,7 @@ clblasStatus clblasAmdQuantizeRows(clblasAmdType type, size_t M, size_t K, const
     if (!valid_type(type)) return clblasInvalidValue;
     CBA_CHECK(check_rows(M, K, ldx, MAT_A, X, offX, size_of(type)));
     CBA_CHECK(check_rows(M, K, ldq, MAT_C, Q, offQ, 1));
+    CBA_CHECK(check_scales(scale, M, true));
     if (M > kMaxDim || K > kMaxDim || !strides_in_range({ldx, ldq})) return clblasNotImplemented;
     return map_hip_error(cba::ffn::quantize_rows(type, (int)M, (int)K, mat(X, offX, ldx, size_of(type)), reinterpret_cast<int8_t *>(Q) + offQ,
                                                  (int64_t)ldq, scale, stream));
@@ -81,6 +91,8 @@ clblasStatus clblasAmdI8gemm(clblasAmdType typeC, size_t M, size_t N, size_t K, 
     CBA_CHECK(check_rows(M, K, lda, MAT_A, A, offA, 1));
     CBA_CHECK(check_rows(N, K, ldb, MAT_B, B, offB, 1));
     CBA_CHECK(check_rows(M, N, ldc, MAT_C, C, offC, size_of(typeC)));
+    CBA_CHECK(check_scales(scaleA, M, true));
+    CBA_CHECK(check_scales(scaleB, N, false));
     if (M > kMaxDim || N > kMaxDim || K > kMaxDepthI8 || !strides_in_range({lda, ldb, ldc})) return clblasNotImplemented;
     return map_hip_error(cba::with_workspaces_secured(stream, [&] {
         return cba::ffn::product_i8(typeC, 0, (int)M, (int)N, (int)K, mat(A, offA, lda, 1), scaleA, mat(B, offB, ldb, 1), scaleB, Mat(),
@@ -127,6 +139,9 @@ clblasStatus clblasAmdGatedI8(clblasAmdType typeH, clblasAmdGate gate, size_t M,
     CBA_CHECK(check_rows(N, K, ldwg, MAT_B, Wg, offWg, 1));
     CBA_CHECK(check_rows(N, K, ldwu, MAT_B, Wu, offWu, 1));
     CBA_CHECK(check_rows(M, N, ldh, MAT_C, H, offH, size_of(typeH)));
+    CBA_CHECK(check_scales(scaleX, M, true));
+    CBA_CHECK(check_scales(scaleWg, N, false));
+    CBA_CHECK(check_scales(scaleWu, N, false));
     if (M > kMaxDim || N > kMaxDim || K > kMaxDepthI8 || !strides_in_range({ldx, ldwg, ldwu, ldh})) return clblasNotImplemented;
     return map_hip_error(cba::with_workspaces_secured(stream, [&] {
         return cba::ffn::product_i8(typeH, gate, (int)M, (int)N, (int)K, mat(X, offX, ldx, 1), scaleX, mat(Wg, offWg, ldwg, 1), scaleWg,

@@ -414,3 +414,165 @@ def test_on_a_side_stream_beside_the_default_one():
         assert cb.i8gemm(cb.Type.F32, M, N, K, A, 0, K, sa, B, 0, K, sb, C, 0, N, stream=streams[i % 3]) == 0
     torch.cuda.synchronize()
     assert all(torch.equal(outs[0], C) for C in outs[1:])
+
+
+# ---- every form of the kernels, and what the choice of a form leaves to larger calls ----
+
+FORMS = list(range(9))  # four from registers, five tiled
+# tails of every length in a step's 16-byte slots and in its two halves; more tiles than workgroups; few steps per tile
+FORM_SHAPES = [(70, 90, 8, 0), (70, 90, 63, 1), (33, 140, 65, 1), (130, 70, 97, 3), (257, 300, 127, 1), (64, 128, 129, 3), (300, 520, 450, 2), (1500, 1600, 40, 0)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("splits", [0, 3])
+def test_every_form(form, splits):
+    from gpu_util import debug_env
+    with debug_env(CLBLAS_AMD_FFN_FORM=form, CLBLAS_AMD_FFN_SPLITS=splits):
+        for M, N, K, pad in FORM_SHAPES:
+            test_i8gemm(cb.Type.BF16, M, N, K, 0, pad + 3)
+            test_gated(cb.Type.F16, True, M, N, K, 0, pad)
+            test_gated_i8(cb.Type.F32, M, N, K, 0, 4 - (K + 1) % 4)
+            if form >= 4:  # (the gradients are tiled)
+                test_gated_grad(cb.Type.BF16, M, N, K, 0, pad)
+                test_gated_grad(cb.Type.F16, K, M, N, 0, 0)
+
+
+@pytest.mark.parametrize("form", [4, 5, 6, 7, 8])
+@pytest.mark.parametrize("K", [100, 260])
+def test_more_tiles_than_workgroups(form, K):
+    """One or a few steps per tile, and workgroups that walk several tiles: the loads of later tiles run ahead."""
+    from gpu_util import debug_env
+    M, N = (4300, 4500) if form == 4 else (3000, 3100)
+    with debug_env(CLBLAS_AMD_FFN_FORM=form):
+        test_i8gemm(cb.Type.F16, M, N, K, 0, 0)
+        test_gated(cb.Type.BF16, False, M, N // 2 + 7, K, 0, 0)
+        if K == 100:
+            n = 2700 if form == 4 else 1500
+            test_gated_grad(cb.Type.BF16, n, n + 30, n + 8, 0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_what_lies_between_rows_does_not_matter(form):
+    """NaN in the gaps between the rows of every operand, where loads of whole pieces of a row reach."""
+    from gpu_util import debug_env
+    M, N, d = 70, 200, torch.bfloat16
+    for K, pad in ((57, 1), (64, 2), (101, 3), (200, 8)):
+        X, Wg, Wu = (Buf(n, K, d, 0, pad, normal(n, K, i), fill=math.nan) for i, n in enumerate((M, N, N)))
+        G, U, dH = (Buf(M, N, d, 0, pad, normal(M, N, 3 + i), fill=math.nan) for i in range(3))
+        H, dX, dWg, dWu = Buf(M, N, d, 0, pad), Buf(M, K, d, 0, pad), Buf(N, K, d, 0, pad), Buf(N, K, d, 0, pad)
+        with debug_env(CLBLAS_AMD_FFN_FORM=form):
+            assert cb.gated(cb.Type.BF16, cb.Gate.Silu, M, N, K, *X.args(), *Wg.args(), *Wu.args(), *H.args()) == 0
+            assert cb.gated_grad(cb.Type.BF16, cb.Gate.Silu, M, N, K, *dH.args(), *X.args(), *Wg.args(), *Wu.args(), *G.args(), *U.args(), *dX.args(),
+                                 *dWg.args(), *dWu.args()) == 0
+        torch.cuda.synchronize()
+        for b in (H, dX, dWg, dWu):
+            assert bool(torch.isfinite(b.mat).all()) and b.surroundings_untouched()
+
+
+def test_results_and_operands_beyond_32_bits():
+    """Element offsets past 2^31 and byte offsets past 2^32, in operands and results; rows from both ends are checked."""
+    M, N, K = 33000, 66000, 64
+    A, B = whole(M, K, 1).cuda(), whole(N, K, 2).cuda()
+    sa, sb = scales(M, 3).cuda(), scales(N, 4).cuda()
+    C = torch.full((M, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert cb.i8gemm(cb.Type.BF16, M, N, K, A, 0, K, sa, B, 0, K, sb, C, 0, N) == 0
+    torch.cuda.synchronize()
+    for r in (slice(0, 40), slice(16400, 16440), slice(M - 40, M)):
+        want = (A[r].double() @ B.double().t()) * sa[r].double()[:, None] * sb.double()[None, :]
+        close(C[r], want, want.abs() * 3 * 2.0 ** -24, torch.bfloat16)
+    # the result as an operand: rows 132 000 bytes apart
+    ld, m, k, n = N, M, 72, 48
+    Wg, Wu = normal(n, k, 5).bfloat16().cuda(), normal(n, k, 6).bfloat16().cuda()
+    H = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    assert cb.gated(cb.Type.BF16, cb.Gate.Gelu, m, n, k, C, 0, ld, Wg, 0, k, Wu, 0, k, H, 0, n) == 0
+    dX, dWg, dWu = torch.empty(m, k, dtype=torch.bfloat16, device="cuda"), torch.empty_like(Wg), torch.empty_like(Wu)
+    dH, G, U = (normal(m, n, 7 + i).bfloat16().cuda() for i in range(3))
+    assert cb.gated_grad(cb.Type.BF16, cb.Gate.Gelu, m, n, k, dH, 0, n, C, 0, ld, Wg, 0, k, Wu, 0, k, G, 0, n, U, 0, n, dX, 0, k, dWg, 0, k, dWu, 0, k) == 0
+    Q, s = torch.empty(m, k, dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda")
+    assert cb.quantize_rows(cb.Type.BF16, m, k, C, 0, ld, Q, 0, k, s) == 0
+    torch.cuda.synchronize()
+    x = C[:, :k].double()
+    g, u = x @ Wg.double().t(), x @ Wu.double().t()
+    eg, eu = k * SUM * (x.abs() @ Wg.double().abs().t()), k * SUM * (x.abs() @ Wu.double().abs().t())
+    h, eh = gated_want(cb.Gate.Gelu, g, u, eg, eu)
+    close(H, h, eh, torch.bfloat16)
+    a = x.abs().amax(1, keepdim=True)
+    assert torch.equal(Q.double(), torch.where(a > 0, torch.round(127 * x / a), torch.zeros_like(x)))
+    du, dg = dH.double() * act(cb.Gate.Gelu, G.double()), dH.double() * U.double() * slope(cb.Gate.Gelu, G.double())
+    for got, v in ((dWg, dg), (dWu, du)):
+        e = half_step(torch.bfloat16, v) * 1.01 + (dH * U).double().abs() * 2.0 ** -19 + dH.double().abs() * 2.0 ** -19
+        close(got, v.t() @ x, e.t() @ x.abs() + m * SUM * (v.abs().t() @ x.abs()), torch.bfloat16)
+
+
+def test_same_weights_twice_and_no_copy_of_results():
+    """Wg and Wu the same matrix: H = act(G) o G."""
+    M, N, K = 50, 60, 70
+    X, W = normal(M, K, 1).half().cuda(), (normal(N, K, 2) / 8).half().cuda()
+    H, G, U = (torch.empty(M, N, dtype=torch.float16, device="cuda") for _ in range(3))
+    assert cb.gated(cb.Type.F16, cb.Gate.Silu, M, N, K, X, 0, K, W, 0, K, W, 0, K, H, 0, N, G, 0, N, U, 0, N) == 0
+    assert torch.equal(G, U)
+    g = X.double() @ W.double().t()
+    e = K * SUM * (X.double().abs() @ W.double().abs().t())
+    h, eh = gated_want(cb.Gate.Silu, g, g, e, e)
+    close(H, h, eh, torch.float16)
+
+
+def test_repeated_calls_give_the_same_bits():
+    for M, N, K in ((16, 700, 4096), (100, 90, 8200), (513, 771, 1030)):
+        a = [t.clone() for t in _outs(M, N, K)]
+        for _ in range(3):
+            assert all(torch.equal(x, y) for x, y in zip(a, _outs(M, N, K)))
+
+
+def _outs(M, N, K):
+    bufs = grad_case(cb.Type.BF16, cb.Gate.Gelu, M, N, K, 0, 0)
+    H = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    assert cb.gated(cb.Type.BF16, cb.Gate.Gelu, M, N, K, *bufs[0].args(), *bufs[1].args(), *bufs[2].args(), H, 0, N) == 0
+    torch.cuda.synchronize()
+    return [H] + [b.mat for b in bufs[6:]]
+
+
+def test_reserved_workspace_lets_the_first_call_be_captured():
+    """The sizes that the header gives are enough."""
+    M, N, K = 100, 90, 8201  # copies (rows of an odd number of 16-bit elements) and partial sums
+    d = torch.bfloat16
+    X, Wg, Wu = (normal(n, K, i).to(d).cuda() for i, n in enumerate((M, N, N)))
+    G, U, dH = (normal(M, N, 3 + i).to(d).cuda() for i in range(3))
+    H, dX, dWg, dWu = torch.empty(M, N, dtype=d, device="cuda"), torch.empty_like(X), torch.empty_like(Wg), torch.empty_like(Wu)
+    row = (2 * K + 127) // 128 * 128
+    copies = row * (M + 2 * N) + 3 * 256
+    grads = 4 * M * ((N + 63) // 64 * 64) + copies + 256
+    sums = 32 * 4 * max(2 * M * (N + 3), M * (K + 3) + 2 * N * (K + 3)) + 256
+    stream = torch.cuda.Stream()
+    assert cb.reserve_workspace(gemm_bytes=sums, trmm_bytes=max(copies, grads), stream=stream) == 0
+    torch.cuda.synchronize()
+
+    def run():
+        a = cb.gated(cb.Type.BF16, cb.Gate.Silu, M, N, K, X, 0, K, Wg, 0, K, Wu, 0, K, H, 0, N)
+        b = cb.gated_grad(cb.Type.BF16, cb.Gate.Silu, M, N, K, dH, 0, N, X, 0, K, Wg, 0, K, Wu, 0, K, G, 0, N, U, 0, N, dX, 0, K, dWg, 0, K, dWu, 0, K)
+        return a, b
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert run() == (0, 0)
+    graph.replay()
+    torch.cuda.synchronize()
+    first = [t.clone() for t in (H, dX, dWg, dWu)]
+    assert run() == (0, 0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, (H, dX, dWg, dWu)))
+
+
+def test_memory_check_covers_the_scales():
+    from gpu_util import debug_env
+    A, B, C = torch.zeros(4, 16, dtype=torch.int8, device="cuda"), torch.zeros(600, 16, dtype=torch.int8, device="cuda"), torch.zeros(4, 600, device="cuda")
+    big = torch.ones(1 << 20, device="cuda")
+    end = big[-2:]  # (allocations are rounded up: only the end of one is known to be an end)
+    with debug_env(CLBLAS_AMD_CHECK_MEM=1):
+        assert cb.i8gemm(cb.Type.F32, 4, 600, 16, A, 0, 16, big, B, 0, 16, big, C, 0, 600) == 0
+        ok = cb.i8gemm(cb.Type.F32, 1, 600, 16, A, 0, 16, end, B, 0, 16, big, C, 0, 600)
+        assert ok == 0
+        far = big.data_ptr() + (1 << 40)
+        assert cb.i8gemm(cb.Type.F32, 4, 600, 16, A, 0, 16, far, B, 0, 16, big, C, 0, 600) == cb.Status.InvalidVecX
+        assert cb.i8gemm(cb.Type.F32, 4, 600, 16, A, 0, 16, big, B, 0, 16, far, C, 0, 600) == cb.Status.InvalidVecY
+    torch.cuda.synchronize()
