@@ -259,28 +259,49 @@ Tiling cut_depth(Tiling c, int tile, bool gated, int M, int N, int splits) {
     return c;
 }
 
-// Time (us) of a launch over tilings that share it: the steps that the busiest of 256 CUs goes through, about 4.5 us for the
-// launch, the first loads and the results, and for sums in pieces a second launch (3 us) and the partial sums, written and
-// read again, at 0.6 us per MB (256 x 4096 x 4096 gated in two ranges of 64 x 128 tiles: 16.8 MB, 43.5 us; in one, 36.7).
-// memory: us that the operands take from memory.  Tilings that share a launch share the CUs: then a workgroup's own steps take as
-// long as its CU needs for one of each of its workgroups (the deepest tiles end last).
+// How `grid` workgroups are shared out between two lists of tiles: so that the busiest has the fewest steps to do.
+struct Share {
+    int blocks = 0;     // for the first list
+    int64_t steps = 0;  // of the busiest workgroup
+};
+Share share_out(const Tiling *c, int grid) {
+    Share best;
+    const uint32_t n0 = (uint32_t)c[0].count(), n1 = (uint32_t)c[1].count();
+    if (n0 == 0 || n1 == 0 || n0 + n1 <= (uint32_t)grid) {
+        const uint32_t n = n0 ? n0 : n1;
+        best.blocks = (int)(n0 < (uint32_t)grid ? n0 : (uint32_t)grid);
+        const int64_t s0 = n0 ? c[0].steps_per_split : 0, s1 = n1 ? c[1].steps_per_split : 0;
+        best.steps = n0 && n1 ? (s0 > s1 ? s0 : s1) : (int64_t)((n + grid - 1) / (uint32_t)grid) * (n0 ? s0 : s1);
+        return best;
+    }
+    for (uint32_t rounds = (n0 + grid - 2) / (uint32_t)(grid - 1), tries = 0; rounds <= n0 && tries < 64; ++rounds, ++tries) {
+        const uint32_t blocks = (n0 + rounds - 1) / rounds, others = grid - blocks;
+        const int64_t s0 = (int64_t)rounds * c[0].steps_per_split, s1 = (int64_t)((n1 + others - 1) / others) * c[1].steps_per_split;
+        const int64_t steps = s0 > s1 ? s0 : s1;
+        if (best.steps && steps >= best.steps && s0 > s1) break;
+        if (!best.steps || steps < best.steps) {
+            best.blocks = (int)blocks;
+            best.steps = steps;
+        }
+    }
+    return best;
+}
+
+// Time (us) of a launch over the tiles of one product (n = 1) or two: the steps that the busiest workgroup goes through, 4.5 us
+// for the launch, the first loads and the results, and for sums in pieces a second launch (3 us) and the partial sums, written
+// and read again, at 0.6 us per MB (256 x 4096 x 4096 gated in two ranges of 64 x 128 tiles: 16.8 MB, 43.5 us; in one, 36.7).
+// memory: us that the operands take from memory.
 double tiled_cost(int tile, const Tiling *c, int n, double memory) {
     const TileShape &t = kTiles[tile];
-    double count = 0, steps = 0, longest = 0, partial = 0;
-    for (int i = 0; i < n; ++i) {
-        count += (double)c[i].count();
-        steps += (double)c[i].count() * c[i].steps_per_split;
-        if (c[i].count() && c[i].steps_per_split > longest) longest = c[i].steps_per_split;
-        partial += (double)c[i].ws_bytes;
-    }
-    double time;
-    if (count <= 256) time = longest * t.step_alone;
-    else if (n == 1) time = (double)(((int64_t)count + 255) >> 8) * longest * t.step_busy;
-    else {
-        const double own = longest * (t.log_bm + t.log_bn <= 14 ? 2 : 1) * t.step_busy, all = steps / 256 * t.step_busy;
-        time = own > all ? own : all;
-    }
+    const int64_t count = c[0].count() + (n > 1 ? c[1].count() : 0);
+    const int per_cu = t.log_bm + t.log_bn <= 14 ? 2 : 1;
+    int64_t steps;
+    if (n > 1) steps = share_out(c, 256 * per_cu).steps;
+    else steps = count <= 256 ? c[0].steps_per_split : ((count + 255) >> 8) * c[0].steps_per_split;
+    // (a workgroup that shares its CU goes through a step in the time of two)
+    double time = steps * (count <= 256 ? t.step_alone : n > 1 ? per_cu * t.step_busy : t.step_busy);
     if (time < memory) time = memory;
+    const double partial = (double)c[0].ws_bytes + (n > 1 ? (double)c[1].ws_bytes : 0.0);
     return 4.5 + time + (partial > 0 ? 3.0 + partial * 0.6e-6 : 0.0);
 }
 
@@ -294,22 +315,22 @@ struct Choice {
 };
 
 // From registers: what the busiest CU reads, at 33 bytes per ns (measured for workgroups of 16 x 16 ... 64 x 32 results,
-// gated and 8-bit, 16 ... 256 rows; within 10 %), or the weights from memory at 5.4 TB/s; 2.8 us for the launch.
-double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes, double memory) {
-    const int64_t groups = ceil_div(M, 16 * s.tm) * ceil_div(N, 16 * s.tn);
+// gated and 8-bit, 16 ... 256 rows; within 10 %; 20 where rows have to be shifted into place), or the weights from memory at 5.4 TB/s; 2.8 us for the launch.
+double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes, double memory, bool shift) {
+    const int64_t groups = (int64_t)((uint32_t)(M + 16 * s.tm - 1) / (16u * s.tm)) * ((uint32_t)(N + 16 * s.tn - 1) / (16u * s.tn));
     const int64_t rows = (M < 16 * s.tm ? M : 16 * s.tm) + 16 * s.tn * (gated ? 2 : 1);
-    const double cu = (double)ceil_div(groups, 256) * rows * k_bytes / 33e3;
+    const double cu = (double)((groups + 255) >> 8) * rows * k_bytes / (shift ? 20e3 : 33e3);
     return 2.8 + (cu > memory ? cu : memory);
 }
 
 // copied: bytes that a tiled form would have to copy first (0.4 us per MB and a launch), where the registers form reads
 // anything as it is.  tiled: whether the rows are short enough for the tiled forms.
-Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool tiled) {
+Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool tiled, bool shift) {
     Choice best;
     const double memory = ((double)M + (double)N * (gated ? 2 : 1)) * k_bytes / 5.4e6;
     const int forced = knobs().ffn_form;
     for (int i = 0; i < ROWS_FORMS; ++i) {
-        const double cost = rows_cost(kRows[i], gated, M, N, k_bytes, memory);
+        const double cost = rows_cost(kRows[i], gated, M, N, k_bytes, memory, shift);
         if (forced >= 0 ? forced == i || (!tiled && i == 0) : cost < best.cost) {
             best.form = i;
             best.cost = cost;
@@ -390,12 +411,12 @@ template <typename Cfg> hipError_t launch_rows(Product p, int K, hipStream_t str
     return launched("ffn_rows_kernel", type_letter(Cfg::ET), 16 * Cfg::TM, 16 * Cfg::TN, Cfg::THREADS, p.M, p.N, K, (unsigned)grid, 1, 1, e);
 }
 
-template <int ET, bool GATED> hipError_t run_rows(const Product &p, int form, int K, hipStream_t stream) {
+template <int ET, bool GATED, bool SHIFT> hipError_t run_rows(const Product &p, int form, int K, hipStream_t stream) {
     switch (form) {
-    case 0: return launch_rows<RowsCfg<ET, 1, 1, 8, 4, GATED>>(p, K, stream);
-    case 1: return launch_rows<RowsCfg<ET, 2, 1, 8, 4, GATED>>(p, K, stream);
-    case 2: return launch_rows<RowsCfg<ET, 2, 2, 8, 2, GATED>>(p, K, stream);
-    default: return launch_rows<RowsCfg<ET, 4, 2, 4, 2, GATED>>(p, K, stream);
+    case 0: return launch_rows<RowsCfg<ET, 1, 1, 8, SHIFT ? 3 : 4, GATED, SHIFT>>(p, K, stream);
+    case 1: return launch_rows<RowsCfg<ET, 2, 1, 8, SHIFT ? 2 : 4, GATED, SHIFT>>(p, K, stream);
+    case 2: return launch_rows<RowsCfg<ET, 2, 2, 8, SHIFT ? 1 : 2, GATED, SHIFT>>(p, K, stream);
+    default: return launch_rows<RowsCfg<ET, 4, 2, 4, SHIFT ? 1 : 2, GATED, SHIFT>>(p, K, stream);
     }
 }
 
@@ -442,7 +463,9 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
         copy[i] = !fits(ptr[i], ld[i]);
         if (copy[i]) at[i] = copies.add((size_t)kp * rows[i]);
     }
-    const Choice c = choose(GATED, M, N, kb, (int64_t)copies.used, kp <= kMaxRowBytes);
+    bool shift = false;  // some row does not start on a dword
+    for (int i = 0; i < OPERANDS; ++i) shift |= ((reinterpret_cast<uintptr_t>(ptr[i]) | (uintptr_t)ld[i]) & 3) != 0;
+    const Choice c = choose(GATED, M, N, kb, (int64_t)copies.used, kp <= kMaxRowBytes, shift);
     const bool tiled = c.form >= ROWS_FORMS;
     char *buf = nullptr;
     uint32_t *ws = nullptr;
@@ -471,24 +494,19 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
     p.k_bytes = kb;
     p.M = M;
     p.N = N;
-    if (!tiled) return run_rows<ET, GATED>(p, c.form, K, stream);
+    if (!tiled) return shift ? run_rows<ET, GATED, true>(p, c.form, K, stream) : run_rows<ET, GATED, false>(p, c.form, K, stream);
     return run_tiles<ET, GATED>(tiled_product(p, c.tiling, ws), c.form - ROWS_FORMS, K, stream);
 }
 
-// The two products of the gradient in one launch.  The workgroups are shared out by the steps there are to do; a product that
-// is not wanted has no tiles.
+// The two products of the gradient in one launch.  A product that is not wanted has no tiles.
 template <int ET> hipError_t run_two(const Product &px, const Product &pw, const Tiling *c, int tile, int M, int N, int K, hipStream_t stream) {
     const int64_t nx = c[0].count(), nw = c[1].count();
     if (nx > 0x3fffffff || nw > 0x3fffffff) return hipErrorNotSupported;
     hipError_t e = with_tile<ET, false, ALONG_K, ACROSS_K>(tile, [&](auto cfg) {
         typedef decltype(cfg) Cfg0;
         typedef TileCfg<ET, Cfg0::BM, Cfg0::BN, Cfg0::WM, Cfg0::WN, Cfg0::S, false, ACROSS_K, ACROSS_K> Cfg1;
-        const double wx = (double)nx * c[0].steps_per_split, ww = (double)nw * c[1].steps_per_split;
         int64_t grid = nx + nw < resident<Cfg0>() ? nx + nw : resident<Cfg0>();
-        int64_t blocks = nx + nw <= grid ? nx : (int64_t)(grid * wx / (wx + ww) + 0.5);
-        if (nx && blocks < 1) blocks = 1;
-        if (nw && blocks > grid - 1) blocks = grid - 1;
-        if (blocks > nx) blocks = nx;
+        const int64_t blocks = share_out(c, (int)grid).blocks;
         if (grid - blocks > nw) grid = blocks + nw;
         auto kernel = two_tiles_kernel<Cfg0, Cfg1>;
         hipError_t e = ensure_dynamic_lds((const void *)kernel, Cfg0::LDS);

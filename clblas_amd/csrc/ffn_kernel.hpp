@@ -324,7 +324,7 @@ template <typename Cfg> static __device__ __forceinline__ TileAt tile_at(Args &p
 // 16-bit result.  ALONG_K: quad j holds columns 16 j + 4 g on; lanes 16 apart exchange halves (v_permlane16_swap), after which
 // an even lane group g has columns 4 g .. 4 g + 7 of block j and its odd neighbour those of block j + 1, and a store writes
 // 64 bytes of each of 16 rows.  (8 bytes per lane: 32 bytes a row, 16 x more often half a cache line; gated 8192 x
-// 12288 x 4096 with G and U stored @STORE@.)  ACROSS_K: element e of a quad comes from the e-th block of a group, and two quads
+// 12288 x 4096 with G and U stored 1330 us, this 1273.)  ACROSS_K: element e of a quad comes from the e-th block of a group, and two quads
 // are neighbours anyway.
 template <typename Cfg> struct Results {
     typedef Fragments<Cfg::BM, Cfg::LAYA, Cfg::TM> FragA;
@@ -700,10 +700,12 @@ template <typename Cfg0, typename Cfg1> __global__ __launch_bounds__(Cfg0::THREA
 // a tile of 16 TM x 16 TN (GATED: 16 TN channels of both weights), and its W waves share the DEPTH, wave w taking every
 // W-th piece of 128 bytes.  So no wave needs what another has loaded: each reads its rows from memory straight into the
 // MFMAs' registers, DEEP pieces ahead, without a barrier, and the W partial tiles are added up in LDS once at the end
-// (in wave order).  Loads need no alignment; rows behind the last one are read as the last one, and not stored.
-template <int ET_, int TM_, int TN_, int W_, int DEEP_, bool GATED_> struct RowsCfg {
+// (in wave order).  Rows behind the last one are read as the last one, and not stored.
+// SHIFT: rows that do not all start on a dword.  Unaligned 16-byte loads take 2.5 times as long (6 x 536 x 7503 gated in 51 us), so
+// each is made from aligned dwords, one more than the four, and shifted into place by bytes (v_alignbyte_b32).
+template <int ET_, int TM_, int TN_, int W_, int DEEP_, bool GATED_, bool SHIFT_> struct RowsCfg {
     static constexpr int ET = ET_, TM = TM_, TN = TN_, W = W_, DEEP = DEEP_;
-    static constexpr bool GATED = GATED_;
+    static constexpr bool GATED = GATED_, SHIFT = SHIFT_;
     static constexpr int NB = GATED ? 2 * TN : TN;  // blocks of weights' rows
     static constexpr int THREADS = 64 * W;
     static constexpr int PITCH = 16 * NB + 4;        // of a partial tile's row in LDS, 32-bit sums
@@ -758,24 +760,55 @@ template <typename Cfg> __global__ __launch_bounds__(Cfg::THREADS, 2) void rows_
         b[j] = static_cast<const char *>(p.B[h]) + (int64_t)(n < p.N ? n : p.N - 1) * p.ldb[h];
     }
     sx4 acc[TM][NB] = {};
-    u32x4 fa[D][TM][2], fb[D][NB][2];
+    // 16 bytes as they come: four dwords, and with SHIFT the one behind them - or the fourth again where the row is aligned and the
+    // fifth need not exist.
+    struct Raw {
+        u32x4 v;
+        uint32_t more;
+    };
+    Raw fa[D][TM][2], fb[D][NB][2];
+    // (off: where in a dword the row starts, and so every piece of it)
+    auto fetch = [&](const char *row, int64_t at) {
+        Raw f;
+        if constexpr (Cfg::SHIFT) {
+            const uint32_t off = (uint32_t)(uintptr_t)row & 3;
+            const char *from = static_cast<const char *>(__builtin_assume_aligned(row - off, 4)) + at;
+            __builtin_memcpy(&f.v, __builtin_assume_aligned(from, 4), 16);
+            __builtin_memcpy(&f.more, __builtin_assume_aligned(from + (off ? 16 : 12), 4), 4);
+        } else {
+            __builtin_memcpy(&f.v, __builtin_assume_aligned(row + at, 4), 16);
+        }
+        return f;
+    };
+    auto operand = [&](const Raw &f, const char *row) {
+        if constexpr (!Cfg::SHIFT) return f.v;
+        const uint32_t off = (uint32_t)(uintptr_t)row & 3;
+        return u32x4{__builtin_amdgcn_alignbyte(f.v[1], f.v[0], off), __builtin_amdgcn_alignbyte(f.v[2], f.v[1], off),
+                     __builtin_amdgcn_alignbyte(f.v[3], f.v[2], off), __builtin_amdgcn_alignbyte(f.more, f.v[3], off)};
+    };
     auto load = [&](int d, int piece) {
         const int64_t at = (int64_t)piece * 128 + g * 16;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) __builtin_memcpy(&fb[d][j][kk], b[j] + at + 64 * kk, 16);
+            for (int j = 0; j < NB; ++j) fb[d][j][kk] = fetch(b[j], at + 64 * kk);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) __builtin_memcpy(&fa[d][i][kk], a[i] + at + 64 * kk, 16);
+            for (int i = 0; i < TM; ++i) fa[d][i][kk] = fetch(a[i], at + 64 * kk);
         }
     };
     auto use = [&](int d) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int kk = 0; kk < 2; ++kk) {
+            u32x4 vb[NB];
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+            for (int j = 0; j < NB; ++j) vb[j] = operand(fb[d][j][kk], b[j]);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) acc[i][j] = Op::run(fb[d][j][kk], fa[d][i][kk], acc[i][j]);
+            for (int i = 0; i < TM; ++i) {
+                const u32x4 va = operand(fa[d][i][kk], a[i]);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = Op::run(vb[j], va, acc[i][j]);
+            }
+        }
     };
     // pieces wave, wave + W, ... of the whole ones are this wave's
     const int whole = (int)(p.k_bytes >> 7), mine = whole > wave ? (whole - wave + W - 1) / W : 0;
