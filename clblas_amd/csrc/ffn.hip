@@ -35,9 +35,9 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(con
     constexpr int KEEP = 4;
     struct Vec8 { T v[8]; };
     __shared__ uint32_t part[4];
-    for (int row = blockIdx.x; row < M; row += gridDim.x) {
-        const T *x = X + (int64_t)row * ldx;
-        int8_t *q = Q + (int64_t)row * ldq;
+    for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {  // (row + 2^20 may pass 31 bits)
+        const T *x = X + row * ldx;
+        int8_t *q = Q + row * ldq;
         const int vecs = K / 8;
         Vec8 kept[KEEP];
         // magnitudes compare as integers, and a NaN's is the largest
@@ -318,6 +318,7 @@ struct Choice {
 // gated and 8-bit, 16 ... 256 rows; within 10 %; 20 where rows have to be shifted into place), or the weights from memory at 5.4 TB/s; 2.8 us for the launch.
 double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes, double memory, bool shift) {
     const int64_t groups = (int64_t)((uint32_t)(M + 16 * s.tm - 1) / (16u * s.tm)) * ((uint32_t)(N + 16 * s.tn - 1) / (16u * s.tn));
+    if (groups >= 1 << 23) return 1e29;  // (of 512 threads: more than one launch holds)
     const int64_t rows = (M < 16 * s.tm ? M : 16 * s.tm) + 16 * s.tn * (gated ? 2 : 1);
     const double cu = (double)((groups + 255) >> 8) * rows * k_bytes / (shift ? 20e3 : 33e3);
     return 2.8 + (cu > memory ? cu : memory);

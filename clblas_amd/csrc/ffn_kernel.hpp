@@ -35,12 +35,12 @@ template <> struct ElemOf<ET_BF16> { typedef __bf16 type; typedef float Acc; };
 // One MFMA on 16 x 16 blocks, 64 bytes deep.  Lane l holds row l % 16 of either operand, the 16 bytes from byte
 // 16 (l / 16) of the depth on; of the result it holds column l % 16, rows 4 (l / 16) .. + 3.
 template <int ET> struct Mfma;
-#define CBA_FFN_MFMA(ET, ACC, OPND, BUILTIN)                                                              \
-    template <> struct Mfma<ET> {                                                                         \
-        typedef ACC Acc;                                                                                      \
-        static __device__ __forceinline__ Acc run(u32x4 a, u32x4 b, Acc c) {                                  \
-            return BUILTIN(__builtin_bit_cast(OPND, a), __builtin_bit_cast(OPND, b), c, 0, 0, 0);             \
-        }                                                                                                     \
+#define CBA_FFN_MFMA(ET, ACC, OPND, BUILTIN)                                                            \
+    template <> struct Mfma<ET> {                                                                       \
+        typedef ACC Acc;                                                                                \
+        static __device__ __forceinline__ Acc run(u32x4 a, u32x4 b, Acc c) {                            \
+            return BUILTIN(__builtin_bit_cast(OPND, a), __builtin_bit_cast(OPND, b), c, 0, 0, 0);       \
+        }                                                                                               \
     };
 CBA_FFN_MFMA(ET_I8, i32x4, i32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8)
 CBA_FFN_MFMA(ET_F16, f32x4, f16x8, __builtin_amdgcn_mfma_f32_16x16x32_f16)
@@ -257,7 +257,7 @@ template <int X, Lay LAY, int NBLK> struct Fragments {
     static __device__ __forceinline__ uint32_t halves(uint32_t row, uint32_t next_row, int e) {
         return __builtin_amdgcn_perm(next_row, row, e & 1 ? 0x07060302u : 0x05040100u);
     }
-    // f: the V registers quadruples of one group
+    // f: the V quadruples of registers of one group
     static __device__ __forceinline__ void ready(u32x4 *f) {
         if constexpr (V == 4) {
             u32x4 o[4];

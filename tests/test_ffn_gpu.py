@@ -576,3 +576,30 @@ def test_memory_check_covers_the_scales():
         assert cb.i8gemm(cb.Type.F32, 4, 600, 16, A, 0, 16, far, B, 0, 16, big, C, 0, 600) == cb.Status.InvalidVecX
         assert cb.i8gemm(cb.Type.F32, 4, 600, 16, A, 0, 16, big, B, 0, 16, far, C, 0, 600) == cb.Status.InvalidVecY
     torch.cuda.synchronize()
+
+
+def test_quantize_rows_more_rows_than_31_bits_can_step_over():
+    """Rows numbered up to almost 2^31: the step from a workgroup's row to its next one passes 31 bits."""
+    M = 2 ** 31 - 600
+    X = torch.full((M,), 2.0, dtype=torch.bfloat16, device="cuda")
+    X[-3:] = torch.tensor([0.0, -4.0, 8.0], device="cuda")
+    Q, s = torch.zeros(M + 8, dtype=torch.int8, device="cuda"), torch.zeros(M, device="cuda")
+    assert cb.quantize_rows(cb.Type.BF16, M, 1, X, 0, 1, Q, 0, 1, s) == 0
+    torch.cuda.synchronize()
+    assert Q[-11:].tolist() == [0, -127, 127] + [0] * 8 and s[-4:].tolist() == [torch.tensor(v / 127).float().item() for v in (2.0, 0.0, 4.0, 8.0)]
+    assert bool((Q[:M - 3] == 127).all()) and bool((s[:M - 3] == s[0]).all())
+
+
+def test_more_rows_than_one_launch_of_the_smallest_products_holds():
+    """2^29 tokens, one channel: a register form's grid would pass 2^32 threads."""
+    M = 2 ** 29 + 77
+    A = torch.ones(M, 4, dtype=torch.int8, device="cuda")
+    A[::1000003, 2] = 3
+    sa = torch.full((M,), 0.5, device="cuda")
+    B, sb = torch.ones(1, 4, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda")
+    C = torch.zeros(M + 4, dtype=torch.float16, device="cuda")
+    assert cb.i8gemm(cb.Type.F16, M, 1, 4, A, 0, 4, sa, B, 0, 4, sb, C, 0, 1) == 0
+    torch.cuda.synchronize()
+    want = torch.full((M,), 2.0, dtype=torch.float16, device="cuda")
+    want[::1000003] = 3.0
+    assert torch.equal(C[:M], want) and not C[M:].any()
