@@ -335,14 +335,17 @@ clblasStatus clblasZhemm(clblasOrder order, clblasSide side, clblasUplo uplo, si
  * All matrices are row-major: a row of X, H, dH, dX is one token, a row of a weight one channel (the layout in which
  * a linear layer keeps them), `ld` counts the elements from one row to the next, and element offsets are added to the
  * pointers as everywhere in this library.  (Column-major callers of the 8-bit product exchange A with B and M with N: the
- * row-major result of that call is theirs.)  Elements need only the alignment of their type; rows whose addresses
- * and lengths are multiples of 16 bytes spare a copy of that operand into the stream's trmm buffer.  Sums are held
- * in 32 bits - float, or int32 for 8-bit operands - and every result is rounded once, to nearest.  Results must not
- * overlap operands or each other.
+ * row-major result of that call is theirs.)  Elements need only the alignment of their type; an operand whose rows do
+ * not all start on multiples of 4 bytes, or lie more than 4 MB apart, is copied into the stream's trmm buffer by the calls
+ * that go through LDS (the larger ones).  Rows of whole 128-byte lines are read fastest (others cost about a fifth).  Sums are
+ * held in 32 bits - float, or int32 for 8-bit operands - and every result is rounded once, to nearest.  Results must not
+ * overlap operands or each other; what lies between their rows keeps its values.  One call's bits are the same every time.
  * Checks, in this order: null matrices (X, A: clblasInvalidMatA, weights and other operands: ...MatB, results: ...MatC),
  * null scales (clblasInvalidVecX for tokens, ...VecY for channels), types and gates that do not exist or that the call
  * does not take (clblasInvalidValue), zero dimensions (clblasInvalidDim), then leading dimensions, in the order of the
- * arguments (clblasInvalidLeadDim{A,B,C}). ---- */
+ * arguments (clblasInvalidLeadDim{A,B,C}).  Dimensions beyond 2^31 - 513 and leading dimensions beyond 2^31 are refused
+ * with clblasNotImplemented; nothing is enqueued by a call that is refused.  With CLBLAS_AMD_CHECK_MEM=1 the memory behind every
+ * matrix is looked at as in the other calls, and behind the scales (clblasInsufficientMemVecX / VecY). ---- */
 
 typedef enum clblasAmdType_ CLBLAS_AMD_ENUM_BASE {
     clblasAmdF32 = 0,
@@ -392,7 +395,8 @@ clblasStatus clblasAmdGatedI8(clblasAmdType typeH, clblasAmdGate gate, size_t M,
 /* Gradients of the gated product from dH, its operands and the G and U it stored:
  *   dU = dH o act(G),  dG = dH o U o act'(G);   dX = dG Wg + dU Wu,   dWg = dG^T X,   dWu = dU^T X
  * all of `type` (F16 or Bf16).  dG and dU pass through the stream's trmm buffer, rounded to `type` once.  dX may be null (it
- * is not computed), and so may dWg and dWu together; all three null, or one of dWg and dWu alone, is clblasInvalidMatC. */
+ * is not computed), and so may dWg and dWu together; all three null, or one of dWg and dWu alone, is clblasInvalidMatC.
+ * N beyond 2^20 - 320 and K beyond 2^21 - 576 (whose rows would pass 4 MB) are refused with clblasNotImplemented. */
 clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M, size_t N, size_t K,
                                 const void *dH, size_t offdH, size_t lddh, const void *X, size_t offX, size_t ldx,
                                 const void *Wg, size_t offWg, size_t ldwg, const void *Wu, size_t offWu, size_t ldwu,
@@ -424,6 +428,11 @@ clblasStatus clblasAmdReleaseStream(hipStream_t stream);
  *               (N rounded up to 64, times N elements) of a rank-k update - SYRK, SYR2K, HERK,
  *               HER2K - of a small C with a deep K (N <= 704 and K >= 4096), which also takes
  *               gemm_bytes for its K ranges;
+ *               The products of a gated feed-forward layer: gemm_bytes for partial sums, 4 bytes for every result
+ *               (two for each of a gated product's, rows rounded up to 4) in every range of K, ranges and tiles
+ *               together at most 512 tiles of 256 x 256 (the gradients 2048); trmm_bytes for copies of operands
+ *               (rows rounded up to 128 bytes, each operand to 256) and, the gradients, for [dG | dU]: 4 M N bytes, N
+ *               rounded up to 64;
  *   trsm_bytes  TRSM's packed diagonal blocks (real types: 135 168 elements per 512 rows of the
  *               triangle or part thereof; complex types: 104 448 real elements per 256 rows).
  * A later call on the stream whose needs fit allocates nothing, so it can be the first thing recorded
