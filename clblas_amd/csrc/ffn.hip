@@ -19,7 +19,7 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // q = round_half_even(127 x / a), a the row's largest magnitude, exactly: the quotient is formed in float (off by at
 // most 127 (2^-24 + 2^-24) < 1.6e-5), and where that lands nearer to a half than it can be off, 254 |x| and
 // (2 n + 1) a are compared in double, where both are exact.  (Halves are no rarity: x = a / 2 is one in every format.)
-// One workgroup per row; a row of up to 8192 elements stays in registers between the two passes.
+// One workgroup per row, or with WAVE one wave; a row of up to 8192 (2048) elements stays in registers between the two passes.
 static __device__ __forceinline__ float quantized(float x, float a, float inv) {
     const float t = fabsf(x) * inv;
     float n = rintf(t);
@@ -31,11 +31,12 @@ static __device__ __forceinline__ float quantized(float x, float a, float inv) {
     return copysignf(n, x);
 }
 
-template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(const T *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scale, int M, int K) {
-    constexpr int KEEP = 4;
+template <typename T, bool WAVE> __global__ __launch_bounds__(256) void quantize_kernel(const T *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scale, int M, int K) {
+    constexpr int KEEP = 4, LANES = WAVE ? 64 : 256, ROWS = 256 / LANES;
+    const int lane = threadIdx.x % LANES;
     struct Vec8 { T v[8]; };
     __shared__ uint32_t part[4];
-    for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {  // (row + 2^20 may pass 31 bits)
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < M; row += gridDim.x * ROWS) {  // (row + 2^20 may pass 31 bits)
         const T *x = X + row * ldx;
         int8_t *q = Q + row * ldq;
         const int vecs = K / 8;
@@ -48,32 +49,34 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(con
         };
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) {
-            const int c = threadIdx.x + i * 256;
+            const int c = lane + i * LANES;
             if (c < vecs) {
                 __builtin_memcpy(&kept[i], x + (int64_t)c * 8, sizeof(Vec8));
 #pragma unroll
                 for (int e = 0; e < 8; ++e) take(kept[i].v[e]);
             }
         }
-        for (int c = threadIdx.x + KEEP * 256; c < vecs; c += 256) {
+        for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
             Vec8 v;
             __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
 #pragma unroll
             for (int e = 0; e < 8; ++e) take(v.v[e]);
         }
-        const int tail = vecs * 8 + threadIdx.x;
+        const int tail = vecs * 8 + lane;
         if (tail < K) take(x[tail]);
 #pragma unroll
         for (int d = 32; d; d >>= 1) {
             const uint32_t o = __shfl_xor(top, d);
             top = o > top ? o : top;
         }
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-        __syncthreads();
+        if (!WAVE) {
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = part[w] > top ? part[w] : top;
+            for (int w = 0; w < 4; ++w) top = part[w] > top ? part[w] : top;
+        }
         float a = __builtin_bit_cast(float, top);
-        if (threadIdx.x == 0) scale[row] = a / 127.f;
+        if (lane == 0) scale[row] = a / 127.f;
         // tiny rows are scaled up first (exact), so that 127 / a stays finite; a row without a finite, positive a is zero
         const float up = a < 0x1p-100f ? 0x1p100f : 1.f;
         a *= up;
@@ -88,16 +91,16 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(con
         };
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) {
-            const int c = threadIdx.x + i * 256;
+            const int c = lane + i * LANES;
             if (c < vecs) eight(kept[i], c);
         }
-        for (int c = threadIdx.x + KEEP * 256; c < vecs; c += 256) {
+        for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
             Vec8 v;
             __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
             eight(v, c);
         }
         if (tail < K) q[tail] = one(x[tail]);
-        __syncthreads();  // (the next row's parts)
+        if (!WAVE) __syncthreads();  // (the next row's parts)
     }
 }
 
@@ -623,13 +626,24 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
 
 }  // namespace
 
+template <typename T, bool WAVE>
+static hipError_t run_quantize(int M, int K, const void *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scale, char type, hipStream_t stream) {
+    const int64_t groups = WAVE ? ceil_div(M, 4) : M;
+    const dim3 grid((unsigned)(groups < (1 << 20) ? groups : 1 << 20));
+    const hipError_t e = launch_kernel(quantize_kernel<T, WAVE>, grid, dim3(256), 0, stream, static_cast<const T *>(X), ldx, Q, ldq, scale, M, K);
+    return launched("ffn_quantize_kernel", type, WAVE ? 4 : 1, K, 256, M, 1, K, grid.x, 1, 1, e);
+}
+template <typename T> static hipError_t quantize_as(int M, int K, Mat X, int8_t *Q, int64_t ldq, float *scale, char type, hipStream_t stream) {
+    // Short rows in great number get a wave each instead of a workgroup: the launch of the workgroups is the time (bf16, us, a
+    // workgroup / a wave a row: 16384 x 64 21 / 8, x 1000 26 / 14, x 2048 28 / 24, x 4096 42 / 49; 4096 x 1000 8.3 / 5.7, x 2048
+    // 9.1 / 9.2; up to 1024 rows no difference below 1000, 4.2 / 7.1 at 2048).
+    if (K <= 1024 && M >= 2048) return run_quantize<T, true>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
+    return run_quantize<T, false>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
+}
 hipError_t quantize_rows(int type, int M, int K, Mat X, int8_t *Q, int64_t ldq, float *scale, hipStream_t stream) {
-    hipError_t e;
-    const dim3 grid((unsigned)(M < (1 << 20) ? M : 1 << 20)), block(256);
-    if (type == OT_F32) e = launch_kernel(quantize_kernel<float>, grid, block, 0, stream, (const float *)X.ptr, X.ld, Q, ldq, scale, M, K);
-    else if (type == OT_F16) e = launch_kernel(quantize_kernel<_Float16>, grid, block, 0, stream, (const _Float16 *)X.ptr, X.ld, Q, ldq, scale, M, K);
-    else e = launch_kernel(quantize_kernel<__bf16>, grid, block, 0, stream, (const __bf16 *)X.ptr, X.ld, Q, ldq, scale, M, K);
-    return launched("ffn_quantize_kernel", type == OT_F32 ? 's' : type == OT_F16 ? 'h' : 'b', 1, K, 256, M, 1, K, grid.x, 1, 1, e);
+    if (type == OT_F32) return quantize_as<float>(M, K, X, Q, ldq, scale, 's', stream);
+    if (type == OT_F16) return quantize_as<_Float16>(M, K, X, Q, ldq, scale, 'h', stream);
+    return quantize_as<__bf16>(M, K, X, Q, ldq, scale, 'b', stream);
 }
 
 hipError_t product_i8(int out_type, int gate, int M, int N, int K, Mat A, const float *sA, Mat Bg, const float *sBg, Mat Bu,

@@ -54,6 +54,17 @@ def test_quantize_rows(type_, M, K, off, pad):
 
 
 @pytest.mark.parametrize("type_", list(cb.Type))
+@pytest.mark.parametrize("M,K,off,pad", [(2048, 1, 0, 0), (5003, 130, 1, 3), (2051, 1024, 0, 0), (4099, 1023, 1, 0), (4098, 7, 0, 1)])
+def test_quantize_many_short_rows(type_, M, K, off, pad):
+    x = normal(M, K, 7 * M + K)
+    x[5::97] = 0
+    X, q, s = quantize(x, type_, off, pad)
+    a = X.abs().amax(1, keepdim=True)
+    assert torch.equal(q.double(), torch.where(a > 0, torch.round(127 * X / a), torch.zeros_like(X)))
+    assert bool(((s.double() - a[:, 0] / 127).abs() <= 2.0 ** -24 * a[:, 0] / 127 + 2.0 ** -150).all())
+
+
+@pytest.mark.parametrize("type_", list(cb.Type))
 def test_quantize_rows_ties_go_to_even(type_):
     # a = 127 / 8: every x = (n + 1/2) / 8 is a tie; a = 96 and 250: only a / 2 is one (63.5 -> 64)
     n = torch.arange(-127, 127, dtype=torch.float32)
