@@ -502,7 +502,7 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
     return run_tiles<ET, GATED>(tiled_product(p, c.tiling, ws), c.form - ROWS_FORMS, K, stream);
 }
 
-// The two products of the gradient in one launch.  A product that is not wanted has no tiles.
+// The two products of the gradient in one launch.  A product that is not wanted, or not here, has no tiles.
 template <int ET> hipError_t run_two(const Product &px, const Product &pw, const Tiling *c, int tile, int M, int N, int K, hipStream_t stream) {
     const int64_t nx = c[0].count(), nw = c[1].count();
     if (nx > 0x3fffffff || nw > 0x3fffffff) return hipErrorNotSupported;
@@ -524,6 +524,41 @@ template <int ET> hipError_t run_two(const Product &px, const Product &pw, const
     return launched("ffn_join_two_kernel", type_letter(ET), 1, 4, 256, M, N, K, grid.x, 2, px.splits > pw.splits ? px.splits : pw.splits, e);
 }
 
+// Tiles and ranges of depth for one launch over dX's product (M x K, rows of `row` bytes deep), the weights' (N x K twice, M
+// deep) or both; one tile, and ranges of about the same length for both.
+struct GradTiling {
+    Tiling c[2];
+    int tile[2] = {0, 0};
+    double cost = 1e30;
+};
+GradTiling grad_tiling(int M, int N, int K, int64_t row, bool want_x, bool want_w) {
+    GradTiling best;
+    for (int i = 0; i < TILE_FORMS; ++i) {
+        if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
+        Tiling whole[2];
+        if (want_x) whole[0] = tiling(i, false, M, K, 1, row);
+        if (want_w) whole[1] = tiling(i, false, N, K, 2, (int64_t)M * 2);
+        const int longest = whole[0].steps_per_split > whole[1].steps_per_split ? whole[0].steps_per_split : whole[1].steps_per_split;
+        for (int cut : kSplits) {
+            const int fs = knobs().ffn_splits;
+            if (cut > 1 && (fs || cut > longest || whole[0].count() + whole[1].count() > 2048)) break;
+            const uint32_t range = (uint32_t)(longest + cut - 1) / (uint32_t)cut;
+            Tiling t[2];
+            for (int j = 0; j < 2; ++j) t[j] = cut_depth(whole[j], i, false, j ? N : M, K, fs ? fs : (int)((whole[j].steps_per_split + range - 1) / range));
+            if (cut > 1 && t[0].count() + t[1].count() > 2048) break;
+            const double cost = tiled_cost(i, t, 2, 0.0);
+            if (cost < best.cost) {
+                best.cost = cost;
+                for (int j = 0; j < 2; ++j) {
+                    best.c[j] = t[j];
+                    best.tile[j] = i;
+                }
+            }
+        }
+    }
+    return best;
+}
+
 template <int ET, int OT>
 hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu, Mat G, Mat U, OutMat dX, OutMat dWg, OutMat dWu,
                    hipStream_t stream) {
@@ -541,32 +576,22 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         copy[i] = used[i] && !fits(in[i].ptr, in[i].ld * 2);
         if (copy[i]) at[i] = copies.add((size_t)rows[i] * ld_copy);
     }
-    // One tile for both products; each cut into ranges of its depth as the model finds best.
-    int tile = 0;
-    Tiling c[2];
-    double best = 1e30;
-    for (int i = 0; i < TILE_FORMS; ++i) {
-        if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
-        Tiling whole[2];
-        if (want_x) whole[0] = tiling(i, false, M, K, 1, row);
-        if (want_w) whole[1] = tiling(i, false, N, K, 2, (int64_t)M * 2);
-        const int longest = whole[0].steps_per_split > whole[1].steps_per_split ? whole[0].steps_per_split : whole[1].steps_per_split;
-        for (int cut : kSplits) {  // into ranges of about the same length for both
-            const int fs = knobs().ffn_splits;
-            if (cut > 1 && (fs || cut > longest || whole[0].count() + whole[1].count() > 2048)) break;
-            const uint32_t range = (uint32_t)(longest + cut - 1) / (uint32_t)cut;
-            Tiling t[2];
-            for (int j = 0; j < 2; ++j) t[j] = cut_depth(whole[j], i, false, j ? N : M, K, fs ? fs : (int)((whole[j].steps_per_split + range - 1) / range));
-            if (cut > 1 && t[0].count() + t[1].count() > 2048) break;
-            const double cost = tiled_cost(i, t, 2, 0.0);
-            if (cost < best) {
-                best = cost;
-                tile = i;
-                c[0] = t[0];
-                c[1] = t[1];
-            }
+    // Both products in one launch, or each in its own where their sizes ask for different tiles and ranges (few tokens: dX is all
+    // depth, the weights' gradients all results; us, together / apart: 1 x 12288 x 4096 191 / 112, 8 x 4096 x 4096 66 / 42, 64 x
+    // 12288 x 4096 237 / 119; but 200 x 4096 x 4096 64 / 69, 509 x 1367 x 770 30 / 36).
+    GradTiling both = grad_tiling(M, N, K, row, want_x, want_w);
+    bool apart = false;
+    if (want_x && want_w) {
+        const GradTiling x = grad_tiling(M, N, K, row, true, false), w = grad_tiling(M, N, K, row, false, true);
+        apart = x.cost + w.cost < both.cost;
+        if (apart) {
+            both.c[0] = x.c[0];
+            both.c[1] = w.c[1];
+            both.tile[0] = x.tile[0];
+            both.tile[1] = w.tile[1];
         }
     }
+    const Tiling *c = both.c;
     char *buf = nullptr;
     uint32_t *ws = nullptr;
     const size_t sums_x = (size_t)round_up((int64_t)c[0].ws_bytes, 256), sums = sums_x + c[1].ws_bytes;
@@ -621,7 +646,10 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         p[i].N = K;
         p[i] = tiled_product(p[i], c[i], i ? ws + sums_x / 4 : ws);
     }
-    return run_two<ET>(p[0], p[1], c, tile, M, N, K, stream);
+    if (!apart) return run_two<ET>(p[0], p[1], c, both.tile[0], M, N, K, stream);
+    const Tiling only_x[2] = {c[0], Tiling()}, only_w[2] = {Tiling(), c[1]};
+    e = run_two<ET>(p[0], Product(), only_x, both.tile[0], M, N, K, stream);
+    return e != hipSuccess ? e : run_two<ET>(Product(), p[1], only_w, both.tile[1], M, N, K, stream);
 }
 
 }  // namespace
