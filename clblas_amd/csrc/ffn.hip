@@ -19,7 +19,7 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // q = round_half_even(127 x / a), a the row's largest magnitude, exactly: the quotient is formed in float (off by at
 // most 127 (2^-24 + 2^-24) < 1.6e-5), and where that lands nearer to a half than it can be off, 254 |x| and
 // (2 n + 1) a are compared in double, where both are exact.  (Halves are no rarity: x = a / 2 is one in every format.)
-// One workgroup per row, or with WAVE one wave; a row of up to 8192 (2048) elements stays in registers between the two passes.
+// One workgroup per row, or with WAVE one wave (no loop over rows: 16384 x 8192 bf16 in 75.5 us without, 87.5 with one); a row of up to 8192 (2048) elements stays in registers between the two passes.
 static __device__ __forceinline__ float quantized(float x, float a, float inv) {
     const float t = fabsf(x) * inv;
     float n = rintf(t);
@@ -36,72 +36,71 @@ template <typename T, bool WAVE> __global__ __launch_bounds__(256) void quantize
     const int lane = threadIdx.x % LANES;
     struct Vec8 { T v[8]; };
     __shared__ uint32_t part[4];
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < M; row += gridDim.x * ROWS) {  // (row + 2^20 may pass 31 bits)
-        const T *x = X + row * ldx;
-        int8_t *q = Q + row * ldq;
-        const int vecs = K / 8;
-        Vec8 kept[KEEP];
-        // magnitudes compare as integers, and a NaN's is the largest
-        uint32_t top = 0;
-        auto take = [&](T v) {
-            const uint32_t b = __builtin_bit_cast(uint32_t, (float)v) & 0x7fffffffu;
-            top = b > top ? b : top;
-        };
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
+    if (row >= M) return;
+    const T *x = X + row * ldx;
+    int8_t *q = Q + row * ldq;
+    const int vecs = K / 8;
+    Vec8 kept[KEEP];
+    // magnitudes compare as integers, and a NaN's is the largest
+    uint32_t top = 0;
+    auto take = [&](T v) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, (float)v) & 0x7fffffffu;
+        top = b > top ? b : top;
+    };
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i) {
-            const int c = lane + i * LANES;
-            if (c < vecs) {
-                __builtin_memcpy(&kept[i], x + (int64_t)c * 8, sizeof(Vec8));
+    for (int i = 0; i < KEEP; ++i) {
+        const int c = lane + i * LANES;
+        if (c < vecs) {
+            __builtin_memcpy(&kept[i], x + (int64_t)c * 8, sizeof(Vec8));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) take(kept[i].v[e]);
-            }
+            for (int e = 0; e < 8; ++e) take(kept[i].v[e]);
         }
-        for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
-            Vec8 v;
-            __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) take(v.v[e]);
-        }
-        const int tail = vecs * 8 + lane;
-        if (tail < K) take(x[tail]);
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const uint32_t o = __shfl_xor(top, d);
-            top = o > top ? o : top;
-        }
-        if (!WAVE) {
-            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 4; ++w) top = part[w] > top ? part[w] : top;
-        }
-        float a = __builtin_bit_cast(float, top);
-        if (lane == 0) scale[row] = a / 127.f;
-        // tiny rows are scaled up first (exact), so that 127 / a stays finite; a row without a finite, positive a is zero
-        const float up = a < 0x1p-100f ? 0x1p100f : 1.f;
-        a *= up;
-        const bool usable = top > 0 && top < 0x7f800000u;
-        const float inv = usable ? 127.f / a : 0.f;
-        auto one = [&](T v) -> int8_t { return usable ? (int8_t)quantized((float)v * up, a, inv) : (int8_t)0; };
-        auto eight = [&](const Vec8 &v, int c) {
-            int8_t o[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = one(v.v[e]);
-            __builtin_memcpy(q + (int64_t)c * 8, o, 8);
-        };
-#pragma unroll
-        for (int i = 0; i < KEEP; ++i) {
-            const int c = lane + i * LANES;
-            if (c < vecs) eight(kept[i], c);
-        }
-        for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
-            Vec8 v;
-            __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
-            eight(v, c);
-        }
-        if (tail < K) q[tail] = one(x[tail]);
-        if (!WAVE) __syncthreads();  // (the next row's parts)
     }
+    for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
+        Vec8 v;
+        __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) take(v.v[e]);
+    }
+    const int tail = vecs * 8 + lane;
+    if (tail < K) take(x[tail]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint32_t o = __shfl_xor(top, d);
+        top = o > top ? o : top;
+    }
+    if (!WAVE) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = part[w] > top ? part[w] : top;
+    }
+    float a = __builtin_bit_cast(float, top);
+    if (lane == 0) scale[row] = a / 127.f;
+    // tiny rows are scaled up first (exact), so that 127 / a stays finite; a row without a finite, positive a is zero
+    const float up = a < 0x1p-100f ? 0x1p100f : 1.f;
+    a *= up;
+    const bool usable = top > 0 && top < 0x7f800000u;
+    const float inv = usable ? 127.f / a : 0.f;
+    auto one = [&](T v) -> int8_t { return usable ? (int8_t)quantized((float)v * up, a, inv) : (int8_t)0; };
+    auto eight = [&](const Vec8 &v, int c) {
+        int8_t o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = one(v.v[e]);
+        __builtin_memcpy(q + (int64_t)c * 8, o, 8);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const int c = lane + i * LANES;
+        if (c < vecs) eight(kept[i], c);
+    }
+    for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
+        Vec8 v;
+        __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
+        eight(v, c);
+    }
+    if (tail < K) q[tail] = one(x[tail]);
 }
 
 // ---- copies that make an operand fit the tiled product ----
@@ -657,14 +656,14 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
 template <typename T, bool WAVE>
 static hipError_t run_quantize(int M, int K, const void *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scale, char type, hipStream_t stream) {
     const int64_t groups = WAVE ? ceil_div(M, 4) : M;
-    const dim3 grid((unsigned)(groups < (1 << 20) ? groups : 1 << 20));
+    const dim3 grid((unsigned)(groups < (1 << 20) ? groups : 1 << 20), (unsigned)ceil_div(groups, 1 << 20));
     const hipError_t e = launch_kernel(quantize_kernel<T, WAVE>, grid, dim3(256), 0, stream, static_cast<const T *>(X), ldx, Q, ldq, scale, M, K);
-    return launched("ffn_quantize_kernel", type, WAVE ? 4 : 1, K, 256, M, 1, K, grid.x, 1, 1, e);
+    return launched("ffn_quantize_kernel", type, WAVE ? 4 : 1, K, 256, M, 1, K, grid.x, grid.y, 1, e);
 }
 template <typename T> static hipError_t quantize_as(int M, int K, Mat X, int8_t *Q, int64_t ldq, float *scale, char type, hipStream_t stream) {
     // Short rows in great number get a wave each instead of a workgroup: the launch of the workgroups is the time (bf16, us, a
-    // workgroup / a wave a row: 16384 x 64 21 / 8, x 1000 26 / 14, x 2048 28 / 24, x 4096 42 / 49; 4096 x 1000 8.3 / 5.7, x 2048
-    // 9.1 / 9.2; up to 1024 rows no difference below 1000, 4.2 / 7.1 at 2048).
+    // workgroup / a wave a row: 16384 x 64 14.0 / 6.6, x 1000 18.4 / 12.6, x 2048 22.4 / 23.1, x 4096 34.7 / 47.5; 4096 x 1000 6.5 /
+    // 5.5, x 2048 7.9 / 9.3; of 1024 rows no difference up to 1000, 4.7 / 7.1 at 2048).
     if (K <= 1024 && M >= 2048) return run_quantize<T, true>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
     return run_quantize<T, false>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
 }
