@@ -430,7 +430,7 @@ clblasStatus clblasAmdReleaseStream(hipStream_t stream);
  *               gemm_bytes for its K ranges;
  *               The products of a gated feed-forward layer: gemm_bytes for partial sums, 4 bytes for every result
  *               (two for each of a gated product's, rows rounded up to 4) in every range of K, ranges and tiles
- *               together at most 512 tiles of 256 x 256 (the gradients 2048); trmm_bytes for copies of operands
+ *               together at most 512 tiles of 256 x 256 (the gradients: 2048 for dX and for the weights'); trmm_bytes for copies of operands
  *               (rows rounded up to 128 bytes, each operand to 256) and, the gradients, for [dG | dU]: 4 M N bytes, N
  *               rounded up to 64;
  *   trsm_bytes  TRSM's packed diagonal blocks (real types: 135 168 elements per 512 rows of the

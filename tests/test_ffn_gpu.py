@@ -252,6 +252,38 @@ def test_gated_grad(type_, M, N, K, off, pad):
     grad_check(type_, gate, M, N, *grad_case(type_, gate, M, N, K, off, pad))
 
 
+@pytest.mark.parametrize("type_", HALVES)
+@pytest.mark.parametrize("M,N,K,off,pad", [(1, 6000, 2100, 0, 0), (3, 5003, 1030, 0, 6), (40, 3000, 4100, 2, 8), (17, 9000, 203, 1, 0)])
+def test_gated_grad_of_few_tokens_and_wide_layers(type_, M, N, K, off, pad):
+    """Sizes at which the two products may go in a launch each; the same call again, captured, gives the same bits."""
+    gate = GATES[(M + N) % 3]
+    bufs = grad_case(type_, gate, M, N, K, off, pad)
+    grad_check(type_, gate, M, N, *bufs)
+    X, Wg, Wu, G, U, dH, dX, dWg, dWu = bufs
+    keep = [b.mat.clone() for b in (dX, dWg, dWu)]
+
+    def run():
+        assert cb.gated_grad(type_, gate, M, N, K, *dH.args(), *X.args(), *Wg.args(), *Wu.args(), *G.args(), *U.args(), *dX.args(), *dWg.args(),
+                             *dWu.args()) == 0
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run()
+    for _ in range(3):
+        for b in (dX, dWg, dWu):
+            b.mat.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(b.mat, k) for b, k in zip((dX, dWg, dWu), keep))
+        assert all(b.surroundings_untouched() for b in (dX, dWg, dWu))
+
+
 @pytest.mark.parametrize("which", ["x", "w"])
 @pytest.mark.parametrize("M,N,K,off,pad", [(1, 1, 1, 0, 0), (70, 130, 200, 0, 0), (33, 65, 17, 1, 3)])
 def test_gated_grad_of_one_side_alone(which, M, N, K, off, pad):
