@@ -57,6 +57,9 @@ class Gate(enum.IntEnum):
     GeluTanh = 2
 
 
+ROUND_TERMS = 0x100  # may be added to the gate of gated_grad (clblasAmdRoundTerms)
+
+
 class Status(enum.IntEnum):
     Success = 0
     InvalidValue = -30
@@ -497,7 +500,8 @@ def gated_i8(typeH, gate, M, N, K, X, offX, ldx, scaleX, Wg, offWg, ldwg, scaleW
 
 def gated_grad(type_, gate, M, N, K, dH, offdH, lddh, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, G, offG, ldg, U,
                offU, ldu, dX, offdX, lddx, dWg, offdWg, lddwg, dWu, offdWu, lddwu, stream=None):
-    """clblasAmdGatedGrad: dX (or None), dWg and dWu (or both None) from dH, the operands and the stored G and U."""
+    """clblasAmdGatedGrad: dX (or None), dWg and dWu (or both None) from dH, the operands and the stored G and U.
+    gate + ROUND_TERMS: dG and dU rounded to 16 bits on their way (half the matrix work, see include/clblas_amd.h)."""
     return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, _addr(dH), offdH, lddh, _addr(X), offX, ldx,
                                              _addr(Wg), offWg, ldwg, _addr(Wu), offWu, ldwu, _addr(G), offG, ldg, _addr(U),
                                              offU, ldu, _addr(dX), offdX, lddx, _addr(dWg), offdWg, lddwg, _addr(dWu),

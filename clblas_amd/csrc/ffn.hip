@@ -135,45 +135,151 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyList list) {
 
 // ---- gradients of the gate ----
 //
-// dG = dH o U o act'(G), dU = dH o act(G), rounded to the operands' 16 bits as the two products that follow take
-// them (each result below sums many of them: the roundings, independent and unbiased, add up to about one more
-// rounding of the result).  A row per token, [dG | dU], either half padded with zeros to a multiple of 64.
-template <int OT> __global__ __launch_bounds__(256) void gate_grad_kernel(const void *dH_, int64_t lddh, const void *G_, int64_t ldg, const void *U_,
-                                                                          int64_t ldu, int M, int N, int gate, void *out_, int64_t half) {
+// dG = dH o U o act'(G), dU = dH o act(G).  The two products that follow take 16-bit operands.  Rounded to one such number these
+// values would carry its error into every result (2.3e-3 of it instead of 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16), so each is kept
+// as the sum of two (TWO): the first truncated, the second what is left, rounded - 16 bits of bf16, 21 of f16.
+// Truncation gives both the same sign, and the second is not left zero: a term times an infinity is then infinite, and no NaN.
+// Twice the matrix work: 8192 x 12288 x 4096 bf16 5.6 ms, with one number 3.0.  A caller may choose that (clblasAmdRoundTerms).
+// f16 would also lose its range (dH U reaches 2^32): all of a call's values are multiplied by one power of two that brings the
+// largest to 2^14 ... 2^15 (exact; what it pushes below 2^-24 is less than 2^-38 of the largest), and the results by its reciprocal.
+template <int OT, bool TWO> struct Terms {
+    uint16_t first[8], second[8];
+    __device__ __forceinline__ void set(int e, float x, float scale) {
+        if (!TWO) {
+            const auto rounded = Store<OT>::of(OT == OT_F16 ? x * scale : x);
+            first[e] = __builtin_bit_cast(uint16_t, rounded);
+            return;
+        }
+        const bool finite = fabsf(x) < __builtin_inff();
+        if (OT == OT_BF16) {
+            const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+            const uint16_t hi = (uint16_t)(bits >> 16);
+            const __bf16 rest = (__bf16)(x - __builtin_bit_cast(float, bits & 0xffff0000u));
+            uint16_t lo = __builtin_bit_cast(uint16_t, rest);
+            if ((lo & 0x7fff) == 0 && fabsf(x) >= 0x1p-110f) lo = (hi & 0x8000) | 0x0080;
+            first[e] = hi;
+            second[e] = finite ? lo : hi;
+        } else {
+            x *= scale;
+            const _Float16 whole = (_Float16)__builtin_amdgcn_cvt_pkrtz(x, 0.f)[0];
+            const uint16_t hi = __builtin_bit_cast(uint16_t, whole);
+            const _Float16 rest = (_Float16)(x - (float)whole);
+            uint16_t lo = __builtin_bit_cast(uint16_t, rest);
+            if ((lo & 0x7fff) == 0 && (hi & 0x7fff)) lo = (hi & 0x8000) | 1;
+            first[e] = hi;
+            second[e] = finite ? lo : hi;
+        }
+    }
+};
+
+// The values lie as [dG], then [dU]: a row per token, padded with zeros to whole lines of 128 bytes; TWO: 32 first terms and their
+// 32 second ones a line.
+struct GateGrad {
+    const void *dH, *G, *U;
+    int64_t lddh, ldg, ldu;
+    int M, N, gate;
+    char *out;
+    int64_t row, plane;  // bytes from token to token, and from dG to dU
+    uint32_t *top;       // f16: the largest magnitude that each workgroup of the first pass met
+    int tops;
+    float *unscale;      // f16: the reciprocal of the common power of two
+};
+
+// dG and dU of channels n .. n + 7 of token m; zeros behind the last channel.
+template <int OT> static __device__ __forceinline__ void gate_grad8(const GateGrad &p, int64_t m, int n, float (&dg)[8], float (&du)[8]) {
     typedef typename Store<OT>::type T;
     struct Vec8 { T v[8]; };
-    const T *dH = static_cast<const T *>(dH_), *G = static_cast<const T *>(G_), *U = static_cast<const T *>(U_);
-    T *out = static_cast<T *>(out_);
-    const int64_t per_row = half >> 3, total = per_row * M;
+    const T *h = static_cast<const T *>(p.dH) + m * p.lddh + n, *g = static_cast<const T *>(p.G) + m * p.ldg + n,
+            *u = static_cast<const T *>(p.U) + m * p.ldu + n;
+    Vec8 vh = {}, vg = {}, vu = {};
+    if (n + 8 <= p.N) {
+        __builtin_memcpy(&vh, h, 16);
+        __builtin_memcpy(&vg, g, 16);
+        __builtin_memcpy(&vu, u, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (n + e < p.N) {
+                vh.v[e] = h[e];
+                vg.v[e] = g[e];
+                vu.v[e] = u[e];
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float act, slope;
+        gate_value_and_slope(p.gate, (float)vg.v[e], act, slope);
+        const float dh = (float)vh.v[e];
+        dg[e] = dh * (float)vu.v[e] * slope;
+        du[e] = dh * act;
+    }
+}
+
+// The largest of the workgroup's 256 values, in every thread.
+static __device__ __forceinline__ uint32_t largest_of_all(uint32_t top) {
+    __shared__ uint32_t part[4];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint32_t o = __shfl_xor(top, d);
+        top = o > top ? o : top;
+    }
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = part[w] > top ? part[w] : top;
+    return top;
+}
+
+// f16, first pass: the largest finite magnitude (as bits, which compare like it).
+__global__ __launch_bounds__(256) void gate_grad_top_kernel(GateGrad p) {
+    const int64_t per_row = (p.N + 7) >> 3, total = per_row * p.M;
+    uint32_t top = 0;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+        const int64_t m = t / per_row;
+        float dg[8], du[8];
+        gate_grad8<OT_F16>(p, m, (int)(t - m * per_row) * 8, dg, du);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            for (const float x : {dg[e], du[e]}) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
+                if (b < 0x7f800000u && b > top) top = b;
+            }
+    }
+    top = largest_of_all(top);
+    if (threadIdx.x == 0) p.top[blockIdx.x] = top;
+}
+
+template <int OT, bool TWO> __global__ __launch_bounds__(256) void gate_grad_kernel(GateGrad p) {
+    float scale = 1.f;
+    if (OT == OT_F16) {
+        uint32_t top = 0;
+        for (int i = threadIdx.x; i < p.tops; i += 256) top = p.top[i] > top ? p.top[i] : top;
+        top = largest_of_all(top);
+        int e = 0;
+        (void)frexpf(__builtin_bit_cast(float, top), &e);  // top = f 2^e, 1/2 <= f < 1
+        e = top == 0 ? 0 : 15 - e > 100 ? 100 : 15 - e;
+        scale = ldexpf(1.f, e);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.unscale = ldexpf(1.f, -e);
+    }
+    const int64_t per_row = p.row >> (TWO ? 5 : 4), total = per_row * p.M;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
         const int64_t m = t / per_row;
         const int n = (int)(t - m * per_row) * 8;
-        const T *h = dH + m * lddh + n, *g = G + m * ldg + n, *u = U + m * ldu + n;
-        Vec8 vh = {}, vg = {}, vu = {}, dg, du;
-        if (n + 8 <= N) {
-            __builtin_memcpy(&vh, h, 16);
-            __builtin_memcpy(&vg, g, 16);
-            __builtin_memcpy(&vu, u, 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (n + e < N) {
-                    vh.v[e] = h[e];
-                    vg.v[e] = g[e];
-                    vu.v[e] = u[e];
-                }
-        }
+        float dg[8], du[8];
+        gate_grad8<OT>(p, m, n, dg, du);
+        Terms<OT, TWO> g, u;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float act, slope;
-            gate_value_and_slope(gate, (float)vg.v[e], act, slope);
-            const float dh = (float)vh.v[e];
-            dg.v[e] = Store<OT>::of(dh * (float)vu.v[e] * slope);
-            du.v[e] = Store<OT>::of(dh * act);
+            g.set(e, dg[e], scale);
+            u.set(e, du[e], scale);
         }
-        T *to = out + m * 2 * half + n;
-        __builtin_memcpy(__builtin_assume_aligned(to, 16), &dg, 16);
-        __builtin_memcpy(__builtin_assume_aligned(to + half, 16), &du, 16);
+        char *to = p.out + m * p.row + (TWO ? (n >> 5) * 128 + (n & 31) * 2 : (int64_t)n * 2);
+        __builtin_memcpy(__builtin_assume_aligned(to, 16), g.first, 16);
+        __builtin_memcpy(__builtin_assume_aligned(to + p.plane, 16), u.first, 16);
+        if (TWO) {
+            __builtin_memcpy(__builtin_assume_aligned(to + 64, 16), g.second, 16);
+            __builtin_memcpy(__builtin_assume_aligned(to + p.plane + 64, 16), u.second, 16);
+        }
     }
 }
 
@@ -218,13 +324,26 @@ struct TileShape { int log_bm, log_bn; double step_alone, step_busy; };
 const TileShape kTiles[TILE_FORMS] = {
     {8, 8, 1.50, 1.62}, {8, 7, 0.87, 0.97}, {7, 7, 0.97, 0.57}, {6, 7, 0.50, 0.375}, {6, 6, 0.36, 0.27}};  // (edges: powers of two)
 
-template <int ET, bool GATED, Lay LA, Lay LB, typename F> hipError_t with_tile(int tile, F &&f) {
+// The gradients' with two numbers for each term (both sides alone, 16 x 16 and 32 x 32 tiles, 1024 ... 4096 channels or tokens).
+const TileShape kTermTiles[TILE_FORMS] = {{8, 8, 1.50, 1.51}, {8, 7, 0.85, 0.92}, {7, 7, 0.55, 0.455}, {6, 7, 0.46, 0.315}, {6, 6, 0.39, 0.25}};
+
+template <int ET, bool GATED, typename F> hipError_t with_tile(int tile, F &&f) {
     switch (tile) {
-    case 0: return f(TileCfg<ET, 256, 256, 128, 64, 2, GATED, LA, LB>());
-    case 1: return f(TileCfg<ET, 256, 128, 64, 64, 3, GATED, LA, LB>());
-    case 2: return f(TileCfg<ET, 128, 128, 64, 64, 2, GATED, LA, LB>());
-    case 3: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED, LA, LB>());
-    default: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED, LA, LB>());
+    case 0: return f(TileCfg<ET, 256, 256, 128, 64, 2, GATED>());
+    case 1: return f(TileCfg<ET, 256, 128, 64, 64, 3, GATED>());
+    case 2: return f(TileCfg<ET, 128, 128, 64, 64, 2, GATED>());
+    case 3: return f(TileCfg<ET, 64, 128, 32, 64, 3, GATED>());
+    default: return f(TileCfg<ET, 64, 64, 32, 32, 5, GATED>());
+    }
+}
+// The gradients'.  (TWO terms: a stage is a quarter or a third smaller, 32 rows of B to 64 bytes of either term of A.)
+template <int ET, bool TWO, typename F> hipError_t with_grad_tile(int tile, F &&f) {
+    switch (tile) {
+    case 0: return f(TileCfg<ET, 256, 256, 128, 64, TWO ? 3 : 2, false, ALONG_K, ACROSS_K, TWO>());
+    case 1: return f(TileCfg<ET, 256, 128, 64, 64, 3, false, ALONG_K, ACROSS_K, TWO>());
+    case 2: return f(TileCfg<ET, 128, 128, 64, 64, TWO ? 3 : 2, false, ALONG_K, ACROSS_K, TWO>());
+    case 3: return f(TileCfg<ET, 64, 128, 32, 64, TWO ? 5 : 3, false, ALONG_K, ACROSS_K, TWO>());
+    default: return f(TileCfg<ET, 64, 64, 32, 32, TWO ? 6 : 5, false, ALONG_K, ACROSS_K, TWO>());
     }
 }
 
@@ -293,8 +412,7 @@ Share share_out(const Tiling *c, int grid) {
 // for the launch, the first loads and the results, and for sums in pieces a second launch (3 us) and the partial sums, written
 // and read again, at 0.6 us per MB (256 x 4096 x 4096 gated in two ranges of 64 x 128 tiles: 16.8 MB, 43.5 us; in one, 36.7).
 // memory: us that the operands take from memory.
-double tiled_cost(int tile, const Tiling *c, int n, double memory) {
-    const TileShape &t = kTiles[tile];
+double tiled_cost(const TileShape &t, const Tiling *c, int n, double memory) {
     const int64_t count = c[0].count() + (n > 1 ? c[1].count() : 0);
     const int per_cu = t.log_bm + t.log_bn <= 14 ? 2 : 1;
     int64_t steps;
@@ -348,7 +466,7 @@ Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool ti
             if (splits > 1 && (fs || whole.count() * splits > 512)) break;  // (more only costs)
             const Tiling t = cut_depth(whole, i, gated, M, N, fs ? fs : splits);
             if (!fs && t.splits != splits) break;
-            const double cost = tiled_cost(i, &t, 1, memory) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
+            const double cost = tiled_cost(kTiles[i], &t, 1, memory) + (copied ? 3.0 + copied * 0.4e-6 : 0.0);
             if (cost < best.cost || (forced >= 0 && best.form != forced)) {
                 best.form = ROWS_FORMS + i;
                 best.tiling = t;
@@ -385,7 +503,7 @@ unsigned join_grid(const Product &p) {
 }
 
 template <int ET, bool GATED> hipError_t run_tiles(const Product &p, int tile, int K, hipStream_t stream) {
-    hipError_t e = with_tile<ET, GATED, ALONG_K, ALONG_K>(tile, [&](auto cfg) {
+    hipError_t e = with_tile<ET, GATED>(tile, [&](auto cfg) {
         typedef decltype(cfg) Cfg;
         const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
         if (tiles > 0x7fffffff - 65536) return hipErrorNotSupported;
@@ -502,12 +620,12 @@ hipError_t product_from(int es, int M, int N, int K, Mat A, Mat B0, Mat B1, Prod
 }
 
 // The two products of the gradient in one launch.  A product that is not wanted, or not here, has no tiles.
-template <int ET> hipError_t run_two(const Product &px, const Product &pw, const Tiling *c, int tile, int M, int N, int K, hipStream_t stream) {
+template <int ET, bool TWO> hipError_t run_two(const Product &px, const Product &pw, const Tiling *c, int tile, int M, int N, int K, hipStream_t stream) {
     const int64_t nx = c[0].count(), nw = c[1].count();
     if (nx > 0x3fffffff || nw > 0x3fffffff) return hipErrorNotSupported;
-    hipError_t e = with_tile<ET, false, ALONG_K, ACROSS_K>(tile, [&](auto cfg) {
+    hipError_t e = with_grad_tile<ET, TWO>(tile, [&](auto cfg) {
         typedef decltype(cfg) Cfg0;
-        typedef TileCfg<ET, Cfg0::BM, Cfg0::BN, Cfg0::WM, Cfg0::WN, Cfg0::S, false, ACROSS_K, ACROSS_K> Cfg1;
+        typedef TileCfg<ET, Cfg0::BM, Cfg0::BN, Cfg0::WM, Cfg0::WN, Cfg0::S, false, ACROSS_K, ACROSS_K, TWO> Cfg1;
         int64_t grid = nx + nw < resident<Cfg0>() ? nx + nw : resident<Cfg0>();
         const int64_t blocks = share_out(c, (int)grid).blocks;
         if (grid - blocks > nw) grid = blocks + nw;
@@ -523,20 +641,20 @@ template <int ET> hipError_t run_two(const Product &px, const Product &pw, const
     return launched("ffn_join_two_kernel", type_letter(ET), 1, 4, 256, M, N, K, grid.x, 2, px.splits > pw.splits ? px.splits : pw.splits, e);
 }
 
-// Tiles and ranges of depth for one launch over dX's product (M x K, rows of `row` bytes deep), the weights' (N x K twice, M
-// deep) or both; one tile, and ranges of about the same length for both.
+// Tiles and ranges of depth for one launch over dX's product (M x K, x_bytes deep), the weights' (N x K twice, w_bytes deep) or
+// both; one tile, and ranges of about the same length for both.
 struct GradTiling {
     Tiling c[2];
     int tile[2] = {0, 0};
     double cost = 1e30;
 };
-GradTiling grad_tiling(int M, int N, int K, int64_t row, bool want_x, bool want_w) {
+GradTiling grad_tiling(const TileShape *tiles, int M, int N, int K, int64_t x_bytes, int64_t w_bytes, bool want_x, bool want_w) {
     GradTiling best;
     for (int i = 0; i < TILE_FORMS; ++i) {
         if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
         Tiling whole[2];
-        if (want_x) whole[0] = tiling(i, false, M, K, 1, row);
-        if (want_w) whole[1] = tiling(i, false, N, K, 2, (int64_t)M * 2);
+        if (want_x) whole[0] = tiling(i, false, M, K, 1, x_bytes);
+        if (want_w) whole[1] = tiling(i, false, N, K, 2, w_bytes);
         const int longest = whole[0].steps_per_split > whole[1].steps_per_split ? whole[0].steps_per_split : whole[1].steps_per_split;
         for (int cut : kSplits) {
             const int fs = knobs().ffn_splits;
@@ -545,7 +663,7 @@ GradTiling grad_tiling(int M, int N, int K, int64_t row, bool want_x, bool want_
             Tiling t[2];
             for (int j = 0; j < 2; ++j) t[j] = cut_depth(whole[j], i, false, j ? N : M, K, fs ? fs : (int)((whole[j].steps_per_split + range - 1) / range));
             if (cut > 1 && t[0].count() + t[1].count() > 2048) break;
-            const double cost = tiled_cost(i, t, 2, 0.0);
+            const double cost = tiled_cost(tiles[i], t, 2, 0.0);
             if (cost < best.cost) {
                 best.cost = cost;
                 for (int j = 0; j < 2; ++j) {
@@ -558,17 +676,18 @@ GradTiling grad_tiling(int M, int N, int K, int64_t row, bool want_x, bool want_
     return best;
 }
 
-template <int ET, int OT>
+const int kTops = 1024;  // workgroups of the pass that finds f16's largest term: what every one of the next pass reads
+template <int ET, int OT, bool TWO>
 hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu, Mat G, Mat U, OutMat dX, OutMat dWg, OutMat dWu,
                    hipStream_t stream) {
-    const int64_t half = round_up(N, 64), row = 2 * half * 2;  // [dG | dU]: elements to dU, bytes to the next token
+    // [dG], [dU]: bytes from token to token, and from one to the other
+    const int64_t row = round_up((int64_t)N * (TWO ? 4 : 2), 128), plane = M * row, w_bytes = (int64_t)M * (TWO ? 4 : 2);
     const bool want_x = dX.ptr, want_w = dWg.ptr;
     // operands that the tiles load as they are, or copies
     Mat in[3] = {X, Wg, Wu};
     const int64_t rows[3] = {M, N, N}, ld_copy = round_up((int64_t)K * 2, 128);
     const bool used[3] = {want_w, want_x, want_x};
     Copies copies;
-    const size_t at_grads = copies.add((size_t)M * row);
     size_t at[3] = {0, 0, 0};
     bool copy[3];
     for (int i = 0; i < 3; ++i) {
@@ -578,10 +697,11 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
     // Both products in one launch, or each in its own where their sizes ask for different tiles and ranges (few tokens: dX is all
     // depth, the weights' gradients all results; us, together / apart: 1 x 12288 x 4096 191 / 112, 8 x 4096 x 4096 66 / 42, 64 x
     // 12288 x 4096 237 / 119; but 200 x 4096 x 4096 64 / 69, 509 x 1367 x 770 30 / 36).
-    GradTiling both = grad_tiling(M, N, K, row, want_x, want_w);
+    const TileShape *tiles = TWO ? kTermTiles : kTiles;
+    GradTiling both = grad_tiling(tiles, M, N, K, 2 * row, w_bytes, want_x, want_w);
     bool apart = false;
     if (want_x && want_w) {
-        const GradTiling x = grad_tiling(M, N, K, row, true, false), w = grad_tiling(M, N, K, row, false, true);
+        const GradTiling x = grad_tiling(tiles, M, N, K, 2 * row, w_bytes, true, false), w = grad_tiling(tiles, M, N, K, 2 * row, w_bytes, false, true);
         apart = x.cost + w.cost < both.cost;
         if (apart) {
             both.c[0] = x.c[0];
@@ -591,13 +711,16 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         }
     }
     const Tiling *c = both.c;
-    char *buf = nullptr;
-    uint32_t *ws = nullptr;
-    const size_t sums_x = (size_t)round_up((int64_t)c[0].ws_bytes, 256), sums = sums_x + c[1].ws_bytes;
-    hipError_t e = workspace_get(stream, copies.used, WS_TRMM, (void **)&buf);
-    if (e == hipSuccess && sums) e = workspace_get(stream, sums, WS_GEMM, (void **)&ws);
+    // the gemm buffer: partial sums of either product, the terms, and for f16 what their scale comes from
+    const int64_t work = M * (row >> (TWO ? 5 : 4));
+    const int tops = OT == OT_F16 ? (int)(ceil_div(work, 256) < kTops ? ceil_div(work, 256) : kTops) : 0;
+    Copies scratch;
+    const size_t at_x = scratch.add(c[0].ws_bytes), at_w = scratch.add(c[1].ws_bytes), at_terms = scratch.add((size_t)(2 * plane));
+    const size_t at_tops = scratch.add((size_t)tops * 4 + 4);
+    char *buf = nullptr, *ws = nullptr;
+    hipError_t e = copies.used ? workspace_get(stream, copies.used, WS_TRMM, (void **)&buf) : hipSuccess;
+    if (e == hipSuccess) e = workspace_get(stream, scratch.used, WS_GEMM, (void **)&ws);
     if (e != hipSuccess) return e;
-    char *grads = buf + at_grads;
     const void *ptr[3];
     int64_t ld[3];
     CopyList list = {};
@@ -608,32 +731,38 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         if (copy[i]) list.c[n++] = Copy{static_cast<const char *>(in[i].ptr), buf + at[i], in[i].ld * 2, (int64_t)K * 2, ld_copy, rows[i]};
     }
     if ((e = copy_rows(list, n, stream)) != hipSuccess) return e;
-    const int64_t work = M * (half / 8);
+    GateGrad gate_grad = {dH.ptr, G.ptr, U.ptr, dH.ld, G.ld, U.ld, M, N, gate, ws + at_terms, row, plane, (uint32_t *)(ws + at_tops), tops,
+                          (float *)(ws + at_tops) + tops};
+    if (OT == OT_F16) {
+        e = launch_kernel(gate_grad_top_kernel, dim3((unsigned)tops), dim3(256), 0, stream, gate_grad);
+        if ((e = launched("ffn_gate_grad_top_kernel", type_letter(ET), 1, 8, 256, M, N, K, (unsigned)tops, 1, 1, e)) != hipSuccess) return e;
+    }
     const unsigned grid = (unsigned)(ceil_div(work, 256) < 8192 ? ceil_div(work, 256) : 8192);
-    e = launch_kernel(gate_grad_kernel<OT>, dim3(grid), dim3(256), 0, stream, dH.ptr, dH.ld, G.ptr, G.ld, U.ptr, U.ld, M, N, gate, (void *)grads, half);
+    e = launch_kernel(gate_grad_kernel<OT, TWO>, dim3(grid), dim3(256), 0, stream, gate_grad);
     if ((e = launched("ffn_gate_grad_kernel", type_letter(ET), 1, 8, 256, M, N, K, grid, 1, 1, e)) != hipSuccess) return e;
-    Product p[2] = {};  // [dG | dU] (M x 2 half) times [Wg; Wu]: the depth runs through Wg's rows, then through Wu's
-    p[0].A[0] = p[0].A[1] = grads;
-    p[0].a_bytes = M * row;
+    Product p[2] = {};  // [dG | dU] times [Wg; Wu]: the depth runs through dG's row and Wg's rows, then through dU's and Wu's
+    p[0].A[0] = p[0].A[1] = gate_grad.out;
+    p[0].a_bytes = 2 * plane;
+    p[0].a_jump = plane - row;
     for (int h = 0; h < 2; ++h) {
         p[0].B[h] = ptr[1 + h];
         p[0].ldb[h] = ld[1 + h];
         p[0].b_bytes[h] = (N - 1) * ld[1 + h] + (int64_t)K * 2;
     }
-    p[0].k_bytes = row;
-    p[0].part_steps = (int)(half / 64);
+    p[0].k_bytes = 2 * row;
+    p[0].part_steps = (int)(row >> 7);
     p[0].C[0] = p[0].C[1] = dX.ptr;
     p[0].ldc[0] = p[0].ldc[1] = dX.ld;
     p[0].M = M;
     // dG^T X and dU^T X: the depth runs through the tokens
     for (int z = 0; z < 2; ++z) {
-        p[1].A[z] = grads + z * half * 2;
+        p[1].A[z] = gate_grad.out + z * plane;
         p[1].B[z] = ptr[0];
         p[1].ldb[z] = ld[0];
         p[1].b_bytes[z] = (M - 1) * ld[0] + (int64_t)K * 2;
     }
-    p[1].a_bytes = M * row - half * 2;
-    p[1].k_bytes = (int64_t)M * 2;
+    p[1].a_bytes = plane;
+    p[1].k_bytes = w_bytes;
     p[1].C[0] = dWg.ptr;
     p[1].C[1] = dWu.ptr;
     p[1].ldc[0] = dWg.ld;
@@ -643,12 +772,13 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         p[i].out_type = OT;
         p[i].lda = row;
         p[i].N = K;
-        p[i] = tiled_product(p[i], c[i], i ? ws + sums_x / 4 : ws);
+        p[i].unscale = gate_grad.unscale;
+        p[i] = tiled_product(p[i], c[i], (uint32_t *)(ws + (i ? at_w : at_x)));
     }
-    if (!apart) return run_two<ET>(p[0], p[1], c, both.tile[0], M, N, K, stream);
+    if (!apart) return run_two<ET, TWO>(p[0], p[1], c, both.tile[0], M, N, K, stream);
     const Tiling only_x[2] = {c[0], Tiling()}, only_w[2] = {Tiling(), c[1]};
-    e = run_two<ET>(p[0], Product(), only_x, both.tile[0], M, N, K, stream);
-    return e != hipSuccess ? e : run_two<ET>(Product(), p[1], only_w, both.tile[1], M, N, K, stream);
+    e = run_two<ET, TWO>(p[0], Product(), only_x, both.tile[0], M, N, K, stream);
+    return e != hipSuccess ? e : run_two<ET, TWO>(Product(), p[1], only_w, both.tile[1], M, N, K, stream);
 }
 
 }  // namespace
@@ -703,8 +833,10 @@ hipError_t gated(int type, int gate, int M, int N, int K, Mat X, Mat Wg, Mat Wu,
 
 hipError_t gated_grad(int type, int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu, Mat G, Mat U, OutMat dX, OutMat dWg,
                       OutMat dWu, hipStream_t stream) {
-    if (type == OT_F16) return grad_of<ET_F16, OT_F16>(gate, M, N, K, dH, X, Wg, Wu, G, U, dX, dWg, dWu, stream);
-    return grad_of<ET_BF16, OT_BF16>(gate, M, N, K, dH, X, Wg, Wu, G, U, dX, dWg, dWu, stream);
+    const bool two = !(gate & ROUND_TERMS);
+    const auto run = type == OT_F16 ? (two ? grad_of<ET_F16, OT_F16, true> : grad_of<ET_F16, OT_F16, false>)
+                                    : (two ? grad_of<ET_BF16, OT_BF16, true> : grad_of<ET_BF16, OT_BF16, false>);
+    return run(gate & ~ROUND_TERMS, M, N, K, dH, X, Wg, Wu, G, U, dX, dWg, dWu, stream);
 }
 
 }  // namespace ffn

@@ -158,7 +158,7 @@ clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M
     if (!X) return clblasInvalidMatA;
     if (!dH || !Wg || !Wu || !G || !U) return clblasInvalidMatB;
     if ((!dX && !dWg) || !dWg != !dWu) return clblasInvalidMatC;
-    if ((type != clblasAmdF16 && type != clblasAmdBf16) || !valid_gate(gate)) return clblasInvalidValue;
+    if ((type != clblasAmdF16 && type != clblasAmdBf16) || !valid_gate((clblasAmdGate)(gate & ~clblasAmdRoundTerms))) return clblasInvalidValue;
     CBA_CHECK(check_rows(M, N, lddh, MAT_B, dH, offdH, 2));
     CBA_CHECK(check_rows(M, K, ldx, MAT_A, X, offX, 2));
     CBA_CHECK(check_rows(N, K, ldwg, MAT_B, Wg, offWg, 2));

@@ -85,7 +85,7 @@ static __device__ __forceinline__ void gate_value_and_slope(int gate, float g, f
     slope = s + c * s * t * dx;
 }
 
-// Rounds to the storage type (to nearest, ties to even); the only rounding below 32 bits on the way to a result.
+// Rounds to the storage type (to nearest, ties to even): the one rounding of a result.
 template <int OT> struct Store;
 template <> struct Store<OT_F32> {
     typedef float type;
@@ -128,10 +128,12 @@ static __device__ __forceinline__ void finish4(Args &p, int z, int m, int n, con
     const int valid = p.N - n;
     float sa = 1.f;
     if (ET == ET_I8) sa = p.scale_a[m];
+    if (ET == ET_F16 && !GATED) sa = *p.unscale;  // (the gradients)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         x[e] = first[e];
         if (GATED) u[e] = second[e];
+        if (ET == ET_F16 && !GATED) x[e] *= sa;
         if (ET == ET_I8 && e < valid) {
             x[e] = x[e] * sa * p.scale_b[0][n + e];
             if (GATED) u[e] = u[e] * sa * p.scale_b[1][n + e];
@@ -176,9 +178,12 @@ static __device__ __forceinline__ int xcd_contiguous(int id, int total) {
 //
 // An operand lies in memory either with its rows along the depth (ALONG_K: the forward products) or across it
 // (ACROSS_K, 16-bit types: a row per depth index, as the gradients meet weights and activations).
+// TERMS (B across the depth): every value of A is the sum of two 16-bit numbers, first terms and second ones of 32 values
+// side by side (64 bytes each).  A step is then 32 deep: its first MFMAs take the first terms, its second ones the others, and
+// both meet the same operands of B, which are read once.
 //   ALONG_K   LDS image: a row of eight 16-byte slots per tile row, slot s of row r in place s ^ (r % 8), so that the
 //             eight rows that one pass of a fragment read touches lie in different banks.
-//   ACROSS_K  LDS image: 64 rows of depth, each the tile's edge long.  A lane reads V neighbouring columns (8 or 4 bytes) of
+//   ACROSS_K  LDS image: 64 rows of depth (TERMS: 32, of A for either term), each the tile's edge long.  A lane reads V neighbouring columns (8 or 4 bytes) of
 //             its 8 rows of depth and swaps 16-bit halves between row pairs (v_perm_b32): that gives it the operands
 //             of V MFMA blocks, block e holding columns e, V + e, 2 V + e ...  (The transposing LDS reads would do
 //             this without the swaps, but the compiler makes each of them wait for every load into LDS that is in
@@ -187,7 +192,7 @@ static __device__ __forceinline__ int xcd_contiguous(int id, int total) {
 // same WN / 2 channels of the other's), so that both factors of a result end up in the same lane.
 enum Lay { ALONG_K = 0, ACROSS_K = 1 };
 
-template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay LAYA_ = ALONG_K, Lay LAYB_ = ALONG_K> struct TileCfg {
+template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay LAYA_ = ALONG_K, Lay LAYB_ = ALONG_K, bool TERMS_ = false> struct TileCfg {
     static constexpr int ET = ET_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
     static constexpr bool GATED = GATED_;
     static constexpr Lay LAYA = LAYA_, LAYB = LAYB_;
@@ -196,11 +201,15 @@ template <int ET_, int BM_, int BN_, int WM_, int WN_, int S_, bool GATED_, Lay 
     static constexpr int CHANNELS = GATED ? BN / 2 : BN;  // columns of the result per tile
     // B in two parts, one after the other along the depth (the gradient of the input: both weights)
     static constexpr bool PARTS = LAYA == ALONG_K && LAYB == ACROSS_K;
+    static constexpr bool TERMS = TERMS_;
+    static constexpr int DEPTH = TERMS ? 32 : 64;  // of a step, 16-bit types
     static constexpr int TM = WM / 16, TN = WN / 16;
-    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // wave-wide loads per step (1 KiB each)
-    static constexpr int STAGE = (BM + BN) * 128;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * (TERMS ? 64 : 128);
+    static constexpr int LA = A_BYTES / 1024 / WAVES, LB = B_BYTES / 1024 / WAVES;  // wave-wide loads per step (1 KiB each)
+    static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int LDS = S * STAGE;
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "rows divide over the waves");
+    static_assert(A_BYTES % (1024 * WAVES) == 0 && B_BYTES % (1024 * WAVES) == 0, "an operand's loads divide over the waves");
+    static_assert(!TERMS || LAYB == ACROSS_K, "");
     static_assert(!GATED || (WN / 2) % 16 == 0, "the halves of a wave's columns are whole blocks, and whole loads");
     static_assert(!GATED || LAYB == ALONG_K, "");
     static_assert(ET != ET_I8 || (LAYA == ALONG_K && LAYB == ALONG_K), "half swaps are for 16-bit types");
@@ -380,6 +389,8 @@ template <typename Cfg> struct Results {
     template <int OT>
     static __device__ __forceinline__ void store(Args &p, const TileAt &t, const Acc (&acc)[Cfg::TM][Cfg::TN], int wm, int wn, int r, int g) {
         const int N = p.N, n = t.n0 + wn * COLUMNS;
+        constexpr bool SCALED = Cfg::LAYB == ACROSS_K && Cfg::ET == ET_F16;  // (the gradients)
+        const float unscale = SCALED ? *p.unscale : 1.f;
         constexpr int FACTORS = Cfg::GATED ? 2 : 1;
         float scale[FACTORS][QUADS][4];  // of the channels
         if (Cfg::ET == ET_I8) {
@@ -406,6 +417,7 @@ template <typename Cfg> struct Results {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[j][e] = (float)q[e];
+                    if (SCALED) x[j][e] *= unscale;
                     if (Cfg::ET == ET_I8) x[j][e] = x[j][e] * sa * scale[0][j][e];
                     if (Cfg::GATED) {
                         u[j][e] = (float)acc[i][j + Cfg::TN / 2][e];
@@ -448,12 +460,15 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     // The lane's place in what it loads.  (The swizzle repeats after as many rows as lie between two loads of a wave.)
     static_assert(Cfg::LAYA == ALONG_K || Cfg::WAVES * ImA::ROWS_PER_LOAD % 16 == 0, "");
     static_assert(Cfg::LAYB == ALONG_K || Cfg::WAVES * ImB::ROWS_PER_LOAD % 16 == 0, "");
-    const int a_slot = ImA::slot_of(wave, lane) * 16, b_slot = ImB::slot_of(wave, lane) * 16;
+    // (TERMS, A's columns across the depth: after 32 first terms their second ones)
+    constexpr bool PAIRS = Cfg::TERMS && Cfg::LAYA == ACROSS_K;
+    const int a_col = ImA::slot_of(wave, lane);
+    const int a_slot = PAIRS ? (a_col >> 2) * 128 + (a_col & 3) * 16 : a_col * 16, b_slot = ImB::slot_of(wave, lane) * 16;
     const int lda = (int)p.lda, ldb[2] = {(int)p.ldb[0], (int)p.ldb[1]};
     const int a_off = ImA::row_of(0, lane) * lda + a_slot;
     const int b_off[2] = {ImB::row_of(0, lane) * ldb[0] + b_slot, ImB::row_of(0, lane) * ldb[1] + b_slot};
-    const int64_t a_step = Cfg::LAYA == ALONG_K ? 128 : 64 * p.lda;
-    const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[0], Cfg::LAYB == ALONG_K ? 128 : 64 * p.ldb[1]};
+    const int64_t a_step = Cfg::LAYA == ALONG_K ? 128 : Cfg::DEPTH * p.lda;
+    const int64_t b_step[2] = {Cfg::LAYB == ALONG_K ? 128 : Cfg::DEPTH * p.ldb[0], Cfg::LAYB == ALONG_K ? 128 : Cfg::DEPTH * p.ldb[1]};
     const char *b_from[2] = {static_cast<const char *>(p.B[0]), static_cast<const char *>(p.B[1])};
     const int64_t b_len[2] = {p.b_bytes[0], p.b_bytes[1]};
     constexpr int kOutside = (int)0x80000000u;
@@ -461,6 +476,7 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     // The feeding side runs S steps ahead of the multiplying one: the next step to load, and its place in memory.
     // (While a step is within a tile the places only move on; no branch chooses between them.)
     const int part_steps = Cfg::PARTS ? p.part_steps : 0;
+    const int64_t a_jump = Cfg::PARTS ? p.a_jump : 0;
     TileAt feed = tile_at<Cfg>(fresh(args), id);
     int feed_id = id, feed_step = 0;
     const char *a_ptr, *b_ptr[2];
@@ -468,7 +484,8 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     int part = 0;
     auto aim_a = [&] {
         Args &p = fresh(args);
-        const int64_t skip = (Cfg::LAYA == ALONG_K ? feed.m0 * p.lda : (int64_t)feed.m0 * 2) + feed.first_step * a_step;
+        const int64_t jump = Cfg::PARTS && feed.first_step >= part_steps ? a_jump : 0;
+        const int64_t skip = (Cfg::LAYA == ALONG_K ? feed.m0 * p.lda : (int64_t)feed.m0 * (PAIRS ? 4 : 2)) + feed.first_step * a_step + jump;
         a_ptr = static_cast<const char *>(p.A[feed.z]) + skip;
         a_left = p.a_bytes - skip;
     };
@@ -499,7 +516,8 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     auto load_a = [&](char *dst, int i) {
         const int q = wave + i * Cfg::WAVES;
         const bool out = (Cfg::LAYA == ALONG_K ? a_slot : 0) >= feed.bytes(feed_step);
-        const int off = a_off + q * ImA::ROWS_PER_LOAD * lda;
+        const int row = q * ImA::ROWS_PER_LOAD;
+        const int off = a_off + (PAIRS ? (row & 31) * lda + (row >> 5) * 64 : row * lda);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(a_ptr, a_left), (lds_void_t *)(dst + q * 1024), 16, out ? kOutside : off, 0, 0, 0);
     };
     auto load_b = [&](char *dst, int i) {
@@ -514,8 +532,9 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     };
     auto feed_on = [&] {
         if (++feed_step < feed.steps) {
-            a_ptr += a_step;
-            a_left -= a_step;
+            const int64_t on = a_step + (Cfg::PARTS && feed.first_step + feed_step == part_steps ? a_jump : 0);
+            a_ptr += on;
+            a_left -= on;
             if constexpr (Cfg::PARTS) {
                 aim_parts();
             } else {
@@ -559,7 +578,7 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
                 for (int i = 0; i < LA; ++i) cut(at, wave + i * Cfg::WAVES, a_slot, bytes);
             if (Cfg::LAYB == ALONG_K)
 #pragma unroll
-                for (int i = 0; i < LB; ++i) cut(at + BM * 128, wave + i * Cfg::WAVES, b_slot, bytes);
+                for (int i = 0; i < LB; ++i) cut(at + Cfg::A_BYTES, wave + i * Cfg::WAVES, b_slot, bytes);
         }
         CBA_FFN_WAIT_LDS();  // also: this wave's fragment reads of the stage that is loaded into next have completed
         asm volatile("" ::: "memory");
@@ -571,10 +590,12 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     FragB rb;
     ra.init(lane, wm * Cfg::WM);
     rb.init(lane, wn * Cfg::WN);
-    u32x4 fa[2][TM], fb[2][TN];  // operands of a step's two MFMAs
+    // operands of a step's two MFMAs (TERMS: fb[0] those of both, fb[1] the next step's as they were read)
+    u32x4 fa[2][TM], fb[2][TN];
     auto read_one = [&](const char *at, int kk, int i) {
-        if (i < TN) fb[kk][i] = rb.read(at + BM * 128, i, kk);
-        else fa[kk][i - TN] = ra.read(at, i - TN, kk);
+        const int b = Cfg::TERMS && kk ? 0 : TN;
+        if (i < b) fb[Cfg::TERMS ? 1 : kk][i] = rb.read(at + Cfg::A_BYTES, i, kk);
+        else fa[kk][i - b] = ra.read(at, i - b, kk);
     };
     Acc acc[TM][TN];
 
@@ -585,7 +606,7 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
 #pragma unroll
         for (int i = 0; i < LA; ++i) load_a(lds + s * Cfg::STAGE, i);
 #pragma unroll
-        for (int i = 0; i < LB; ++i) load_b(lds + s * Cfg::STAGE + BM * 128, i);
+        for (int i = 0; i < LB; ++i) load_b(lds + s * Cfg::STAGE + Cfg::A_BYTES, i);
         feed_on();
     }
     TileAt t = tile_at<Cfg>(fresh(args), id);
@@ -602,13 +623,18 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     auto multiply = [&](int kk, int loads, int reads, auto &&load, auto &&read) {
         constexpr int ROWS = TM > 1 ? TM - 1 : 1;
 #pragma unroll
-        for (int j = 0; j < TN; j += FragB::V) rb.ready(&fb[kk][j]);
+        for (int j = 0; j < TN; j += FragB::V) {
+            if (Cfg::TERMS && kk) break;
+#pragma unroll
+            for (int e = 0; e < FragB::V && Cfg::TERMS; ++e) fb[0][j + e] = fb[1][j + e];
+            rb.ready(&fb[kk][j]);
+        }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             if (i % FragA::V == 0) ra.ready(&fa[kk][i]);
             // the weights are the instruction's first operand: a lane then holds one token's neighbouring channels
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[kk][j], fa[kk][i], acc[i][j]);
+            for (int j = 0; j < TN; ++j) acc[i][j] = Op::run(fb[Cfg::TERMS ? 0 : kk][j], fa[kk][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
             if (i >= ROWS) continue;
 #pragma unroll
@@ -621,10 +647,10 @@ template <typename Cfg> static __device__ __forceinline__ void walk_tiles(Args *
     // half while the next step's first operands are read and the loads of the step S later start into the stage that is free.
     auto step = [&](int next_bytes) {
         char *const next = after(stage), *const free = stage;
-        multiply(0, 0, TM + TN, [&](int) {}, [&](int o) { read_one(free, 1, o); });
+        multiply(0, 0, Cfg::TERMS ? TM : TM + TN, [&](int) {}, [&](int o) { read_one(free, 1, o); });
         CBA_FFN_WAIT_VM((S - 2) * (LA + LB));
         publish(next, next_bytes);
-        multiply(1, LA + LB, TM + TN, [&](int o) { o < LA ? load_a(free, o) : load_b(free + BM * 128, o - LA); },
+        multiply(1, LA + LB, TM + TN, [&](int o) { o < LA ? load_a(free, o) : load_b(free + Cfg::A_BYTES, o - LA); },
                  [&](int o) { read_one(next, 0, o); });
         feed_on();
         stage = next;

@@ -338,8 +338,9 @@ clblasStatus clblasZhemm(clblasOrder order, clblasSide side, clblasUplo uplo, si
  * row-major result of that call is theirs.)  Elements need only the alignment of their type; an operand whose rows do
  * not all start on multiples of 4 bytes, or lie more than 4 MB apart, is copied into the stream's trmm buffer by the calls
  * that go through LDS (the larger ones).  Rows of whole 128-byte lines are read fastest (others cost about a fifth).  Sums are
- * held in 32 bits - float, or int32 for 8-bit operands - and every result is rounded once, to nearest.  Results must not
- * overlap operands or each other; what lies between their rows keeps its values.  One call's bits are the same every time.
+ * held in 32 bits - float, or int32 for 8-bit operands - and every result is rounded once, to nearest (for what the
+ * gradients sum, see there).  Results must not overlap operands or each other; what lies between their rows keeps its values.
+ * One call's bits are the same every time.
  * Checks, in this order: null matrices (X, A: clblasInvalidMatA, weights and other operands: ...MatB, results: ...MatC),
  * null scales (clblasInvalidVecX for tokens, ...VecY for channels), types and gates that do not exist or that the call
  * does not take (clblasInvalidValue), zero dimensions (clblasInvalidDim), then leading dimensions, in the order of the
@@ -358,7 +359,8 @@ typedef enum clblasAmdType_ CLBLAS_AMD_ENUM_BASE {
 typedef enum clblasAmdGate_ CLBLAS_AMD_ENUM_BASE {
     clblasAmdSilu = 0,
     clblasAmdGelu = 1,
-    clblasAmdGeluTanh = 2
+    clblasAmdGeluTanh = 2,
+    clblasAmdRoundTerms = 0x100 /* may be added to a gate in clblasAmdGatedGrad, see there */
 } clblasAmdGate;
 
 /* Rows to 8-bit integers with one scale each:
@@ -394,7 +396,11 @@ clblasStatus clblasAmdGatedI8(clblasAmdType typeH, clblasAmdGate gate, size_t M,
 
 /* Gradients of the gated product from dH, its operands and the G and U it stored:
  *   dU = dH o act(G),  dG = dH o U o act'(G);   dX = dG Wg + dU Wu,   dWg = dG^T X,   dWu = dU^T X
- * all of `type` (F16 or Bf16).  dG and dU pass through the stream's trmm buffer, rounded to `type` once.  dX may be null (it
+ * all of `type` (F16 or Bf16).  dG and dU pass through the stream's gemm buffer as two numbers of `type` each, which hold 16
+ * (Bf16) or 21 (F16) bits of them, in F16 with a power of two common to the call taken out: whether or not F16 could hold them,
+ * they are off by no more than those bits and 2^-38 of the largest.  The gradients' error is that of sums over 32-bit dG and dU.
+ * With clblasAmdRoundTerms added to the gate, dG and dU are rounded to one number of `type` each (in F16 with the same power of
+ * two): half the matrix work, and every summand off by up to 2^-8 (Bf16) or 2^-11 (F16) of itself.  dX may be null (it
  * is not computed), and so may dWg and dWu together; all three null, or one of dWg and dWu alone, is clblasInvalidMatC.
  * N beyond 2^20 - 320 and K beyond 2^21 - 576 (whose rows would pass 4 MB) are refused with clblasNotImplemented. */
 clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M, size_t N, size_t K,
@@ -430,9 +436,9 @@ clblasStatus clblasAmdReleaseStream(hipStream_t stream);
  *               gemm_bytes for its K ranges;
  *               The products of a gated feed-forward layer: gemm_bytes for partial sums, 4 bytes for every result
  *               (two for each of a gated product's, rows rounded up to 4) in every range of K, ranges and tiles
- *               together at most 512 tiles of 256 x 256 (the gradients: 2048 for dX and for the weights'); trmm_bytes for copies of operands
- *               (rows rounded up to 128 bytes, each operand to 256) and, the gradients, for [dG | dU]: 4 M N bytes, N
- *               rounded up to 64;
+ *               together at most 512 tiles of 256 x 256 (the gradients: 2048 for dX and for the weights'), and in the gradients
+ *               for dG and dU too: 8 M N bytes, N rounded up to 32 (with clblasAmdRoundTerms 4 M N, N rounded up to 64), and 5 KB;
+ *               trmm_bytes for copies of operands (rows rounded up to 128 bytes, each operand to 256);
  *   trsm_bytes  TRSM's packed diagonal blocks (real types: 135 168 elements per 512 rows of the
  *               triangle or part thereof; complex types: 104 448 real elements per 256 rows).
  * A later call on the stream whose needs fit allocates nothing, so it can be the first thing recorded
