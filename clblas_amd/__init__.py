@@ -449,60 +449,99 @@ def hemm(prefix, order, side, uplo, M, N, alpha, A, offA, lda, B, offB, ldb, bet
 # ---- the products of a gated feed-forward layer (row-major; include/clblas_amd.h) ----
 # (Calls of a few microseconds: addresses go to ctypes as plain integers.)
 
-def _addr(x):
-    return x if x is None or isinstance(x, int) else x.data_ptr()
+_raw_stream = _current_device = _dtypes = None
 
 
-_raw_stream = None
+def _torch_names():
+    """What the wrappers below need of torch, looked up once."""
+    global _raw_stream, _current_device, _dtypes
+    import torch
+    _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (without asking whether torch has begun)
+    # (current_stream() builds a Stream object: 2.6 us, as long as a launch)
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _dtypes = {Type.F32: torch.float32, Type.F16: torch.float16, Type.BF16: torch.bfloat16, "i8": torch.int8}
 
 
-def _stream_addr(stream, x):
-    """The stream's handle (None: torch's current one on the current device, where tensor x has to live)."""
-    global _raw_stream
+def _dtype(type_, *of):
+    """torch's name for a Type that the call takes; None for another, which the library will refuse."""
+    if _dtypes is None:
+        _torch_names()
+    return _dtypes.get(type_) if type_ in of else None
+
+
+def _addresses(stream, dtypes, *xs):
+    """Addresses of the operands xs - integers, None, or tensors - and the stream's handle behind them (None: torch's current one).
+    Tensors have to live on the current device and hold elements of the type that the call will take them for (integers of
+    its size pass as raw storage)."""
+    device, out = None, []
+    for x, dtype in zip(xs, dtypes):
+        if x is None or isinstance(x, int):
+            out.append(x)
+            continue
+        d = x.get_device()
+        if d != device:
+            if d >= 0 and device is None:
+                device = _current_device()
+            if d != device:
+                raise ValueError("operand on %s, but the current device is a GPU%s" % (x.device, "" if device is None else ", cuda:%d" % device))
+        t = x.dtype
+        if t is not dtype and dtype is not None and (t.is_floating_point or t.is_complex or t.itemsize != dtype.itemsize):
+            raise ValueError("operand of %s where the call takes %s" % (t, dtype))
+        out.append(x.data_ptr())
     if stream is None:
-        import torch
-        device = torch.cuda.current_device()
-        if isinstance(x, torch.Tensor) and x.get_device() != device:
-            raise ValueError("matrix on %s, but the current device is cuda:%d" % (x.device, device))
-        if _raw_stream is None:  # (current_stream() builds a Stream object: 2.6 us, as long as a launch)
-            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
-        return _raw_stream(device)
-    return stream if isinstance(stream, int) else stream.cuda_stream
+        if device is None:
+            import torch
+            device = torch.cuda.current_device()
+        out.append(_raw_stream(device))
+    elif isinstance(stream, int):
+        out.append(stream)
+    else:
+        of = getattr(getattr(stream, "device", None), "index", None)
+        if None not in (of, device) and of != device:
+            raise ValueError("stream of %s, but the current device is cuda:%d" % (stream.device, device))
+        out.append(stream.cuda_stream)
+    return out
 
 
 def quantize_rows(type_, M, K, X, offX, ldx, Q, offQ, ldq, scale, stream=None):
     """clblasAmdQuantizeRows: rows of X (Type) to 8-bit integers Q with one scale each."""
-    return load_library().clblasAmdQuantizeRows(int(type_), M, K, _addr(X), offX, ldx, _addr(Q), offQ, ldq, _addr(scale),
-                                                _stream_addr(stream, X))
+    t = _dtype(type_, Type.F32, Type.F16, Type.BF16)
+    X, Q, scale, stream = _addresses(stream, (t, _dtypes["i8"], _dtypes[0]), X, Q, scale)
+    return load_library().clblasAmdQuantizeRows(int(type_), M, K, X, offX, ldx, Q, offQ, ldq, scale, stream)
 
 
 def i8gemm(typeC, M, N, K, A, offA, lda, scaleA, B, offB, ldb, scaleB, C, offC, ldc, stream=None):
     """clblasAmdI8gemm: C = diag(scaleA) A B^T diag(scaleB), A and B 8-bit, C of typeC (Type)."""
-    return load_library().clblasAmdI8gemm(int(typeC), M, N, K, _addr(A), offA, lda, _addr(scaleA), _addr(B), offB, ldb,
-                                          _addr(scaleB), _addr(C), offC, ldc, _stream_addr(stream, A))
+    t = _dtype(typeC, Type.F32, Type.F16, Type.BF16)
+    q, f = _dtypes["i8"], _dtypes[0]
+    A, scaleA, B, scaleB, C, stream = _addresses(stream, (q, f, q, f, t), A, scaleA, B, scaleB, C)
+    return load_library().clblasAmdI8gemm(int(typeC), M, N, K, A, offA, lda, scaleA, B, offB, ldb, scaleB, C, offC, ldc, stream)
 
 
 def gated(type_, gate, M, N, K, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, H, offH, ldh, G=None, offG=0, ldg=0,
           U=None, offU=0, ldu=0, stream=None):
     """clblasAmdGated: H = act(X Wg^T) o (X Wu^T); G and U (both or neither) receive the two products."""
-    return load_library().clblasAmdGated(int(type_), int(gate), M, N, K, _addr(X), offX, ldx, _addr(Wg), offWg, ldwg,
-                                         _addr(Wu), offWu, ldwu, _addr(H), offH, ldh, _addr(G), offG, ldg, _addr(U), offU,
-                                         ldu, _stream_addr(stream, X))
+    X, Wg, Wu, H, G, U, stream = _addresses(stream, (_dtype(type_, Type.F16, Type.BF16),) * 6, X, Wg, Wu, H, G, U)
+    return load_library().clblasAmdGated(int(type_), int(gate), M, N, K, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, H, offH, ldh,
+                                         G, offG, ldg, U, offU, ldu, stream)
 
 
 def gated_i8(typeH, gate, M, N, K, X, offX, ldx, scaleX, Wg, offWg, ldwg, scaleWg, Wu, offWu, ldwu, scaleWu, H, offH,
              ldh, stream=None):
     """clblasAmdGatedI8: the gated product on 8-bit operands with scales, H of typeH (Type)."""
-    return load_library().clblasAmdGatedI8(int(typeH), int(gate), M, N, K, _addr(X), offX, ldx, _addr(scaleX), _addr(Wg),
-                                           offWg, ldwg, _addr(scaleWg), _addr(Wu), offWu, ldwu, _addr(scaleWu), _addr(H),
-                                           offH, ldh, _stream_addr(stream, X))
+    t = _dtype(typeH, Type.F32, Type.F16, Type.BF16)
+    q, f = _dtypes["i8"], _dtypes[0]
+    X, scaleX, Wg, scaleWg, Wu, scaleWu, H, stream = _addresses(stream, (q, f, q, f, q, f, t), X, scaleX, Wg, scaleWg, Wu, scaleWu, H)
+    return load_library().clblasAmdGatedI8(int(typeH), int(gate), M, N, K, X, offX, ldx, scaleX, Wg, offWg, ldwg, scaleWg, Wu, offWu,
+                                           ldwu, scaleWu, H, offH, ldh, stream)
 
 
 def gated_grad(type_, gate, M, N, K, dH, offdH, lddh, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu, ldwu, G, offG, ldg, U,
                offU, ldu, dX, offdX, lddx, dWg, offdWg, lddwg, dWu, offdWu, lddwu, stream=None):
     """clblasAmdGatedGrad: dX (or None), dWg and dWu (or both None) from dH, the operands and the stored G and U.
     gate + ROUND_TERMS: dG and dU rounded to 16 bits on their way (half the matrix work, see include/clblas_amd.h)."""
-    return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, _addr(dH), offdH, lddh, _addr(X), offX, ldx,
-                                             _addr(Wg), offWg, ldwg, _addr(Wu), offWu, ldwu, _addr(G), offG, ldg, _addr(U),
-                                             offU, ldu, _addr(dX), offdX, lddx, _addr(dWg), offdWg, lddwg, _addr(dWu),
-                                             offdWu, lddwu, _stream_addr(stream, X))
+    dH, X, Wg, Wu, G, U, dX, dWg, dWu, stream = _addresses(stream, (_dtype(type_, Type.F16, Type.BF16),) * 9,
+                                                           dH, X, Wg, Wu, G, U, dX, dWg, dWu)
+    return load_library().clblasAmdGatedGrad(int(type_), int(gate), M, N, K, dH, offdH, lddh, X, offX, ldx, Wg, offWg, ldwg, Wu, offWu,
+                                             ldwu, G, offG, ldg, U, offU, ldu, dX, offdX, lddx, dWg, offdWg, lddwg, dWu, offdWu, lddwu,
+                                             stream)
