@@ -318,6 +318,11 @@ char type_letter(int et) { return et == ET_I8 ? 'i' : et == ET_F16 ? 'h' : 'b'; 
 struct RowsShape { int tm, tn; };
 const RowsShape kRows[] = {{1, 1}, {2, 1}, {2, 2}, {4, 2}};
 enum { ROWS_FORMS = 4, TILE_FORMS = 5 };
+// The form that the debug switch asks for; -1 if it names none.
+int forced_form() {
+    const int form = knobs().ffn_form;
+    return form >= 0 && form < ROWS_FORMS + TILE_FORMS ? form : -1;
+}
 // step: us per step of 128 bytes of depth, alone on a CU / per tile where more tiles than CUs keep it busy.  Measured on products of 128 ... 8192 rows, 1024 ... 12288 channels, 1024 ... 8192 deep (alone: e.g. 64 x 64
 // at 256 x 1024 x 4096 8-bit, 32 steps in 14.9 us; busy: 64 x 128 at 1024 x 4096 x 4096 gated, 4 x 64 steps per CU in 102 us).
 struct TileShape { int log_bm, log_bn; double step_alone, step_busy; };
@@ -449,7 +454,7 @@ double rows_cost(const RowsShape &s, bool gated, int M, int N, int64_t k_bytes, 
 Choice choose(bool gated, int M, int N, int64_t k_bytes, int64_t copied, bool tiled, bool shift) {
     Choice best;
     const double memory = ((double)M + (double)N * (gated ? 2 : 1)) * k_bytes / 5.4e6;
-    const int forced = knobs().ffn_form;
+    const int forced = forced_form();
     for (int i = 0; i < ROWS_FORMS; ++i) {
         const double cost = rows_cost(kRows[i], gated, M, N, k_bytes, memory, shift);
         if (forced >= 0 ? forced == i || (!tiled && i == 0) : cost < best.cost) {
@@ -651,7 +656,7 @@ struct GradTiling {
 GradTiling grad_tiling(const TileShape *tiles, int M, int N, int K, int64_t x_bytes, int64_t w_bytes, bool want_x, bool want_w) {
     GradTiling best;
     for (int i = 0; i < TILE_FORMS; ++i) {
-        if (knobs().ffn_form >= ROWS_FORMS && knobs().ffn_form != ROWS_FORMS + i) continue;
+        if (forced_form() >= ROWS_FORMS && forced_form() != ROWS_FORMS + i) continue;
         Tiling whole[2];
         if (want_x) whole[0] = tiling(i, false, M, K, 1, x_bytes);
         if (want_w) whole[1] = tiling(i, false, N, K, 2, w_bytes);
