@@ -19,7 +19,9 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // q = round_half_even(127 x / a), a the row's largest magnitude, exactly: the quotient is formed in float (off by at
 // most 127 (2^-24 + 2^-24) < 1.6e-5), and where that lands nearer to a half than it can be off, 254 |x| and
 // (2 n + 1) a are compared in double, where both are exact.  (Halves are no rarity: x = a / 2 is one in every format.)
-// One workgroup per row, or with WAVE one wave (no loop over rows: 16384 x 8192 bf16 in 75.5 us without, 87.5 with one); a row of up to 8192 (2048) elements stays in registers between the two passes.
+// One workgroup per row (no loop over rows: 16384 x 8192 bf16 in 75.5 us without, 87.5 with one); up to 8192 elements stay in
+// registers between the two passes, what is behind them is read twice.  WAVE: one wave per row, of kWaveRow elements at most.
+const int kWaveRow = 1024;
 static __device__ __forceinline__ float quantized(float x, float a, float inv) {
     const float t = fabsf(x) * inv;
     float n = rintf(t);
@@ -32,7 +34,7 @@ static __device__ __forceinline__ float quantized(float x, float a, float inv) {
 }
 
 template <typename T, bool WAVE> __global__ __launch_bounds__(256) void quantize_kernel(const T *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scale, int M, int K) {
-    constexpr int KEEP = 4, LANES = WAVE ? 64 : 256, ROWS = 256 / LANES;
+    constexpr int LANES = WAVE ? 64 : 256, ROWS = 256 / LANES, KEEP = WAVE ? kWaveRow / (8 * LANES) : 4;
     const int lane = threadIdx.x % LANES;
     struct Vec8 { T v[8]; };
     __shared__ uint32_t part[4];
@@ -57,7 +59,7 @@ template <typename T, bool WAVE> __global__ __launch_bounds__(256) void quantize
             for (int e = 0; e < 8; ++e) take(kept[i].v[e]);
         }
     }
-    for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
+    for (int c = lane + KEEP * LANES; !WAVE && c < vecs; c += LANES) {
         Vec8 v;
         __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
 #pragma unroll
@@ -95,7 +97,7 @@ template <typename T, bool WAVE> __global__ __launch_bounds__(256) void quantize
         const int c = lane + i * LANES;
         if (c < vecs) eight(kept[i], c);
     }
-    for (int c = lane + KEEP * LANES; c < vecs; c += LANES) {
+    for (int c = lane + KEEP * LANES; !WAVE && c < vecs; c += LANES) {
         Vec8 v;
         __builtin_memcpy(&v, x + (int64_t)c * 8, sizeof(Vec8));
         eight(v, c);
@@ -799,7 +801,7 @@ template <typename T> static hipError_t quantize_as(int M, int K, Mat X, int8_t 
     // Short rows in great number get a wave each instead of a workgroup: the launch of the workgroups is the time (bf16, us, a
     // workgroup / a wave a row: 16384 x 64 14.0 / 6.6, x 1000 18.4 / 12.6, x 2048 22.4 / 23.1, x 4096 34.7 / 47.5; 4096 x 1000 6.5 /
     // 5.5, x 2048 7.9 / 9.3; of 1024 rows no difference up to 1000, 4.7 / 7.1 at 2048).
-    if (K <= 1024 && M >= 2048) return run_quantize<T, true>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
+    if (K <= kWaveRow && M >= 2048) return run_quantize<T, true>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
     return run_quantize<T, false>(M, K, X.ptr, X.ld, Q, ldq, scale, type, stream);
 }
 hipError_t quantize_rows(int type, int M, int K, Mat X, int8_t *Q, int64_t ldq, float *scale, hipStream_t stream) {
