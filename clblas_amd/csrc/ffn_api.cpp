@@ -30,8 +30,8 @@ clblasStatus check_scales(const float *scale, size_t n, bool tokens) {
     return clblasSuccess;
 }
 
-// Byte arithmetic on strides stays in 64 bits: rows * ld * size below 2^63 (no memory is that large, so whatever
-// passes this only has to be addressed correctly).
+// Offsets in elements, rows * ld, stay below 2^63 (and no memory is as large as that: whatever passes this only has to be
+// addressed correctly).
 bool strides_in_range(std::initializer_list<size_t> lds) {
     for (size_t ld : lds)
         if (ld > ((size_t)1 << 31)) return false;
@@ -171,7 +171,7 @@ clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M
         CBA_CHECK(check_rows(N, K, lddwu, MAT_C, dWu, offdWu, 2));
     }
     if (M > kMaxDim || N > kMaxDim || K > kMaxDim ||
-        4 * (N + 63) > (size_t)cba::ffn::kMaxRowBytes || 2 * K + 127 > (size_t)cba::ffn::kMaxRowBytes ||  // rows of [dG | dU] and of copies
+        4 * (N + 63) > (size_t)cba::ffn::kMaxRowBytes || 2 * K + 127 > (size_t)cba::ffn::kMaxRowBytes ||  // rows of dG and dU, and of copies
         !strides_in_range({lddh, ldx, ldwg, ldwu, ldg, ldu, dX ? lddx : 0, dWg ? lddwg : 0, dWg ? lddwu : 0}))
         return clblasNotImplemented;
     return map_hip_error(cba::with_workspaces_secured(stream, [&] {

@@ -402,7 +402,7 @@ clblasStatus clblasAmdGatedI8(clblasAmdType typeH, clblasAmdGate gate, size_t M,
  * With clblasAmdRoundTerms added to the gate, dG and dU are rounded to one number of `type` each (in F16 with the same power of
  * two): half the matrix work, and every summand off by up to 2^-8 (Bf16) or 2^-11 (F16) of itself.  dX may be null (it
  * is not computed), and so may dWg and dWu together; all three null, or one of dWg and dWu alone, is clblasInvalidMatC.
- * N beyond 2^20 - 320 and K beyond 2^21 - 576 (whose rows would pass 4 MB) are refused with clblasNotImplemented. */
+ * N beyond 2^20 - 319 and K beyond 2^21 - 576 (whose rows would pass 4 MB) are refused with clblasNotImplemented. */
 clblasStatus clblasAmdGatedGrad(clblasAmdType type, clblasAmdGate gate, size_t M, size_t N, size_t K,
                                 const void *dH, size_t offdH, size_t lddh, const void *X, size_t offX, size_t ldx,
                                 const void *Wg, size_t offWg, size_t ldwg, const void *Wu, size_t offWu, size_t ldwu,
