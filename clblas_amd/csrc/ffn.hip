@@ -702,7 +702,7 @@ hipError_t grad_of(int gate, int M, int N, int K, Mat dH, Mat X, Mat Wg, Mat Wu,
         if (copy[i]) at[i] = copies.add((size_t)rows[i] * ld_copy);
     }
     // Both products in one launch, or each in its own where their sizes ask for different tiles and ranges (few tokens: dX is all
-    // depth, the weights' gradients all results; us, together / apart: 1 x 12288 x 4096 191 / 112, 8 x 4096 x 4096 66 / 42, 64 x
+    // depth, the weights' gradients all results; us, one number a term, together / apart: 1 x 12288 x 4096 191 / 112, 8 x 4096 x 4096 66 / 42, 64 x
     // 12288 x 4096 237 / 119; but 200 x 4096 x 4096 64 / 69, 509 x 1367 x 770 30 / 36).
     const TileShape *tiles = TWO ? kTermTiles : kTiles;
     GradTiling both = grad_tiling(tiles, M, N, K, 2 * row, w_bytes, want_x, want_w);

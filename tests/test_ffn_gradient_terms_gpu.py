@@ -274,3 +274,30 @@ def test_one_side_alone_equals_a_float_sum_too(type_, which, M, N, K):
         else:
             assert bool((t == 7).all())
     assert which == "x" or bool((dX == 7).all())
+
+
+@pytest.mark.parametrize("type_", HALVES)
+@pytest.mark.parametrize("flags", [0, cb.ROUND_TERMS])
+def test_the_workspace_that_the_header_states_is_enough_and_needed(type_, flags):
+    """Sums in one piece: the gemm buffer holds the terms alone."""
+    from gpu_util import debug_env
+    M, N, K = 2000, 1000, 64
+    need = (4 * M * 1024 if flags else 8 * M * 1024) + 5 * 1024
+    dH, X, Wg, Wu, G, U = layer(type_, M, N, K, 14, w=0.05)
+    dX, dWg, dWu = (torch.full_like(t, 7) for t in (X, Wg, Wu))
+    for bytes_, want in ((need - 16384, cb.Status.InvalidOperation), (need, 0)):
+        stream = torch.cuda.Stream()
+        assert cb.release_stream(stream) == 0
+        assert cb.reserve_workspace(gemm_bytes=bytes_, stream=stream) == 0
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with debug_env(CLBLAS_AMD_FFN_SPLITS=1), torch.cuda.graph(graph, stream=stream):
+            st = cb.gated_grad(type_, cb.Gate.Silu + flags, M, N, K, dH, 0, N, X, 0, K, Wg, 0, K, Wu, 0, K, G, 0, N, U, 0, N, dX, 0, K, dWg, 0, K, dWu, 0, K)
+        assert st == want
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bool((t == 7).all()) == (want != 0) for t in (dX, dWg, dWu))
+        del graph
+        assert cb.release_stream(stream) == 0
+    for got, again in zip((dX, dWg, dWu), gradients(type_, cb.Gate.Silu, dH, X, Wg, Wu, G, U, flags)):
+        assert bool(((got.double() - again.double()).abs() <= again.double().abs() * 2.0 ** -7 + 1e-2).all())
