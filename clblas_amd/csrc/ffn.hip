@@ -140,37 +140,39 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyList list) {
 // dG = dH o U o act'(G), dU = dH o act(G).  The two products that follow take 16-bit operands.  Rounded to one such number these
 // values would carry its error into every result (2.3e-3 of it instead of 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16), so each is kept
 // as the sum of two (TWO): the first truncated, the second what is left, rounded - 16 bits of bf16, 21 of f16.
-// Truncation gives both the same sign, and the second is not left zero: a term times an infinity is then infinite, and no NaN.
+// Truncation gives both the same sign, and neither is left zero: a term times an infinity is then infinite, and no NaN.
 // Twice the matrix work: 8192 x 12288 x 4096 bf16 5.6 ms, with one number 3.0.  A caller may choose that (clblasAmdRoundTerms).
 // f16 would also lose its range (dH U reaches 2^32): all of a call's values are multiplied by one power of two that brings the
 // largest to 2^14 ... 2^15 (exact; what it pushes below 2^-24 is less than 2^-38 of the largest), and the results by its reciprocal.
 template <int OT, bool TWO> struct Terms {
     uint16_t first[8], second[8];
+    static __device__ __forceinline__ float value(uint16_t bits) {
+        return OT == OT_BF16 ? __builtin_bit_cast(float, (uint32_t)bits << 16) : (float)__builtin_bit_cast(_Float16, bits);
+    }
+    static __device__ __forceinline__ uint16_t rounded(float x) {
+        const auto r = Store<OT>::of(x);
+        return __builtin_bit_cast(uint16_t, r);
+    }
+    static __device__ __forceinline__ uint16_t truncated(float x) {
+        if (OT == OT_BF16) return (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
+        const _Float16 r = (_Float16)__builtin_amdgcn_cvt_pkrtz(x, 0.f)[0];
+        return __builtin_bit_cast(uint16_t, r);
+    }
     __device__ __forceinline__ void set(int e, float x, float scale) {
+        if (OT == OT_F16) x *= scale;
         if (!TWO) {
-            const auto rounded = Store<OT>::of(OT == OT_F16 ? x * scale : x);
-            first[e] = __builtin_bit_cast(uint16_t, rounded);
+            first[e] = rounded(x);
             return;
         }
-        const bool finite = fabsf(x) < __builtin_inff();
-        if (OT == OT_BF16) {
-            const uint32_t bits = __builtin_bit_cast(uint32_t, x);
-            const uint16_t hi = (uint16_t)(bits >> 16);
-            const __bf16 rest = (__bf16)(x - __builtin_bit_cast(float, bits & 0xffff0000u));
-            uint16_t lo = __builtin_bit_cast(uint16_t, rest);
-            if ((lo & 0x7fff) == 0 && fabsf(x) >= 0x1p-110f) lo = (hi & 0x8000) | 0x0080;
-            first[e] = hi;
-            second[e] = finite ? lo : hi;
-        } else {
-            x *= scale;
-            const _Float16 whole = (_Float16)__builtin_amdgcn_cvt_pkrtz(x, 0.f)[0];
-            const uint16_t hi = __builtin_bit_cast(uint16_t, whole);
-            const _Float16 rest = (_Float16)(x - (float)whole);
-            uint16_t lo = __builtin_bit_cast(uint16_t, rest);
-            if ((lo & 0x7fff) == 0 && (hi & 0x7fff)) lo = (hi & 0x8000) | 1;
-            first[e] = hi;
-            second[e] = finite ? lo : hi;
+        uint16_t hi = truncated(x), lo = rounded(x - value(hi));
+        if (!(fabsf(x) < __builtin_inff())) {
+            lo = hi;
+        } else if ((lo & 0x7fff) == 0 && (hi & 0x7fff) > 1) {  // one step of the first goes to the second
+            --hi;
+            lo = rounded(x - value(hi));
         }
+        first[e] = hi;
+        second[e] = lo;
     }
 };
 

@@ -301,3 +301,22 @@ def test_the_workspace_that_the_header_states_is_enough_and_needed(type_, flags)
         assert cb.release_stream(stream) == 0
     for got, again in zip((dX, dWg, dWu), gradients(type_, cb.Gate.Silu, dH, X, Wg, Wu, G, U, flags)):
         assert bool(((got.double() - again.double()).abs() <= again.double().abs() * 2.0 ** -7 + 1e-2).all())
+
+
+@pytest.mark.parametrize("size", [2.0 ** 14, 1.0, 2.0 ** -10, 2.0 ** -17, 2.0 ** -26, 2.0 ** -37])
+def test_f16_terms_that_sixteen_bits_hold_stay_exact(size):
+    """One token of a call whose terms are short and `size`, the largest being 2^15, in sums that are short: nothing is added to them.
+    (They are multiplied by 1/2, so from 2^-23 on the smallest f16 holds them; below that they are off by 2^-38 of the largest.)"""
+    d = torch.float16
+    M, N, K = 3, 4, 6
+    f = lambda r, c, v: torch.full((r, c), v, dtype=d, device="cuda")  # noqa: E731
+    dH, U, G = f(M, N, 2.0 ** 8), f(M, N, 2.0 ** 7), f(M, N, 64.0)
+    half = 2.0 ** (math.floor(math.log2(size)) // 2)
+    dH[1], U[1] = half, size / half
+    X, Wg, Wu = f(M, K, 1.0), f(N, K, 0.0), f(N, K, 0.0)
+    Wg[0], Wg[1], Wg[2] = 2.0 ** 13, 2.0 ** 12, 2.0 ** 4
+    dX, _, _ = gradients(cb.Type.F16, cb.Gate.Silu, dH, X, Wg, Wu, G, U)
+    want = size * (2.0 ** 13 + 2.0 ** 12 + 2.0 ** 4)
+    exact = float(torch.tensor(want, dtype=torch.float64).half())
+    off = 0.0 if size >= 2.0 ** -23 else 2.0 ** -38 * 2.0 ** 15 * want / size
+    assert want > 65504 or all(abs(x - exact) <= off for x in dX[1].tolist())
